@@ -391,6 +391,54 @@ int onpu_attn_step_dev(const float *q, int Hq, int D, const void *K, const void 
                        int64_t rs, const float *mask, const float *sinks, float scale, float *out, int kv_bf16,
                        void *stream);
 
+/* ---- 8-bit KV cache: rows of K and V held as int8 codes with one fp32 scale per (sequence, kv head,
+ * block of rows), value = code * scale. No counterpart in the reference (its attention steps read
+ * fp32 / bf16 caches, llama/ggml-opennpu/onpu_cpu.cpp:173-229). All pointers are device memory; the
+ * caller owns the cache and describes it here. */
+typedef struct onpu_kv8_cache {
+    int8_t *k, *v;           /* codes of row j, head h, sequence b at b * bs + h * hs + j * rs, dim of them; */
+                             /* 16-byte aligned, strides multiples of 16, rs >= dim                          */
+    float *k_scale, *v_scale;/* scale of row j at b * sbs + h * shs + j / block                               */
+    int64_t batch, heads, rows, dim;  /* sequences, kv heads, rows a sequence can hold, head size           */
+    int64_t bs, hs, rs;      /* strides of k and v in codes                                                  */
+    int64_t sbs, shs;        /* strides of the scales in floats                                              */
+    int32_t block;           /* rows per scale: 16, 32 or 64                                                 */
+} onpu_kv8_cache;
+/* The calls below work on tokens i = 0 .. cnt[b] - 1 of each sequence b, whose cache rows are pos[b] + i.
+ * pos and cnt are int32 [batch] on the device, so a captured graph is replayed while the sequences
+ * grow; cnt NULL: T everywhere; cnt[b] = 0 leaves sequence b alone. Token rows (k, v, q, out) lie at
+ * (b * T + i) * ld, heads one after another in a row; rows i >= cnt[b] of a padded batch are neither
+ * read nor written. They are bf16 (x_bf16 != 0) or fp32, 16-byte aligned, ld times the element a
+ * multiple of 16 bytes. dim is a multiple of 16, at most 256; batch at most 32767. A sequence whose rows are
+ * not all inside the cache, or whose cnt is not in [0, T], is skipped and sets the device status
+ * (onpu_check_device). Asynchronous on `stream`, no allocation, capturable; calls that touch the same
+ * sequence's rows are ordered by the caller. The device that is current must be the library's.
+ * 0 ok, < 0 error.
+ *
+ * append: quantises rows k, v [batch * T][heads * dim] into the cache. For each block that holds one
+ * of a sequence's new rows: scale = max(old scale, largest |value| of its new rows / 127), the old scale
+ * being 0 when the block holds no row before pos[b]; new codes = the nearest integer (ties to even)
+ * of value / scale, at most +-127; where the scale grew the block's older codes are re-rounded onto
+ * it. An infinite or NaN value makes its block's scale NaN until the block is begun again. */
+int onpu_kv8_append_dev(const onpu_kv8_cache *cache, const void *k, int64_t ldk, const void *v, int64_t ldv, int64_t T,
+                        int x_bf16, const int32_t *pos, const int32_t *cnt, void *stream);
+/* read: cache rows back as code * scale (rounded to fp32, then to the output's type) into k, v
+ * [batch * T][heads * dim]. */
+int onpu_kv8_read_dev(const onpu_kv8_cache *cache, void *k, int64_t ldk, void *v, int64_t ldv, int64_t T, int x_bf16,
+                      const int32_t *pos, const int32_t *cnt, void *stream);
+/* attn: causal softmax attention of q [batch * T][Hq * dim] over the cache, onpu_attn_step's form for batches
+ * and several tokens: query i of sequence b sees rows 0 .. pos[b] + i, query head h reads kv head
+ * h / (Hq / heads) (Hq / heads <= 16); mask fp32 additive, row j for token i of sequence b at
+ * b * mask_bs + i * mask_ts + j (NULL: none; strides may be 0; j below the sequence's pos + cnt is read); sinks
+ * fp32 [Hq] as in onpu_attn_step. Rows whose mask is -inf count for nothing, whatever they hold; a
+ * query that is left no row gives zeros. out: q's layout and type. ws: onpu_kv8_attn_ws bytes of device memory,
+ * 16-byte aligned, used by this call until it is done (calls that run at the same time need one each). */
+int onpu_kv8_attn_dev(const onpu_kv8_cache *cache, const void *q, int64_t ldq, int Hq, int64_t T, int x_bf16,
+                      const int32_t *pos, const int32_t *cnt, const float *mask, int64_t mask_bs, int64_t mask_ts,
+                      const float *sinks, float scale, void *out, int64_t ldo, void *ws, void *stream);
+/* bytes of onpu_kv8_attn_dev's ws for these sizes; < 0 error */
+int64_t onpu_kv8_attn_ws(const onpu_kv8_cache *cache, int Hq, int64_t T, int x_bf16);
+
 /* ---- weight blobs: the GPU layout on disk (replaces what the reference's PackCache stores,
  * npu4/model.py:712-759: the packed upload bytes of one NPU buffer, so a second model load skips
  * reading and quantising the checkpoint). A blob is self-describing: a 64-byte header (magic

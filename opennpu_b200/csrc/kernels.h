@@ -238,4 +238,43 @@ int attn_tile_rows(int D, bool bf16);
 int attn_smem_bytes(int D, int rep, int R, bool bf16);
 cudaError_t attn_launch(const AttnParams &p, bool bf16, cudaStream_t stream);
 
+// ---- 8-bit KV cache (kv8.cu, kv8_attn.cu): int8 codes, one fp32 scale per (sequence, kv head, block of
+// rows), K and V apart; value = code * scale
+struct Kv8Cache {
+    int8_t *k, *v;                    // row j of head h of sequence b at b * bs + h * hs + j * rs (bytes)
+    float *ks, *vs;                   // its scale at b * sbs + h * shs + (j >> blk_log2)
+    int64_t bs, hs, rs, sbs, shs;
+    int B, Hkv, S, D, blk_log2;
+};
+// the rows a call is about: tokens i < cnt[b] (null: T) of sequence b are cache rows pos[b] + i. A
+// sequence whose rows are not all inside the cache, or whose cnt is not in [0, T], is skipped and sets
+// bit 32 of *err.
+struct Kv8Rows {
+    const int32_t *pos, *cnt;
+    int T;
+    int *err;
+};
+// quantise rows k, v (bf16 or fp32, token i of sequence b at (b * T + i) * ld, head h at h * D) into the cache
+cudaError_t kv8_append_launch(const Kv8Cache &c, const Kv8Rows &r, const void *k, int64_t ldk, const void *v,
+                              int64_t ldv, bool bf16, cudaStream_t stream);
+// the other way: cache rows -> k, v in the same layout
+cudaError_t kv8_read_launch(const Kv8Cache &c, const Kv8Rows &r, void *k, int64_t ldk, void *v, int64_t ldv,
+                            bool bf16, cudaStream_t stream);
+struct Kv8AttnParams {
+    Kv8Cache c;
+    Kv8Rows r;
+    const void *q;                    // token i of sequence b at (b * T + i) * ldq, head h at h * D
+    int64_t ldq;
+    void *out;                        // the same layout and type as q
+    int64_t ldo;
+    int Hq;
+    const float *mask;                // additive, row j for token i of sequence b at b * mbs + i * mts + j, or null
+    int64_t mbs, mts;
+    const float *sinks;               // [Hq] or null
+    float scale;
+    void *ws;                         // kv8_attn_ws_bytes, 16-byte aligned
+};
+int64_t kv8_attn_ws_bytes(int Hq, int Hkv, int D, int T, bool bf16);
+cudaError_t kv8_attn_launch(const Kv8AttnParams &p, bool bf16, cudaStream_t stream);
+
 }  // namespace onpu_b200

@@ -410,6 +410,9 @@ int check_device_err(Ctx &c) {
         reset_chains_after_error();
         if (h & 16)
             set_err("an all-reduce timed out waiting for a peer rank (device status %d)", h);
+        else if (h & 32)
+            set_err("rows outside an 8-bit KV cache (pos, cnt) or a cnt outside [0, T]; those sequences were "
+                    "skipped (device status %d)", h);
         else if (h & 8)
             set_err("an expert id was out of range [0, E) in a routed job list; those (token, slot) pairs were "
                     "dropped (device status %d)", h);
@@ -2715,6 +2718,153 @@ int onpu_attn_step_dev(const float *q, int Hq, int D, const void *K, const void 
     std::lock_guard<std::mutex> lk(g_mu);
     return attn_dev(q, Hq, D, K, V, Hkv, S, hs, rs, mask, sinks, scale, out, kv_bf16 != 0,
                     static_cast<cudaStream_t>(stream));
+}
+
+// ------------------------------------------------------------------ 8-bit KV cache
+namespace {
+// What every kv8 call checks first: the cache's description and the token count. Fills c and r.
+bool kv8_check(const char *who, const onpu_kv8_cache *d, int64_t T, const int32_t *pos, const int32_t *cnt,
+               Kv8Cache &c, Kv8Rows &r) {
+    if (!d || !d->k || !d->v || !d->k_scale || !d->v_scale || !pos) {
+        set_err("%s: a null cache, codes, scales or pos pointer", who);
+        return false;
+    }
+    if (d->batch < 1 || d->batch > 32767 || d->heads < 1 || d->heads > 65535 || d->rows < 1 || d->rows > 0x7fffffc0 ||
+        d->dim < 16 || d->dim > 256 || d->dim % 16 || (d->block != 16 && d->block != 32 && d->block != 64)) {
+        set_err("%s: need 1 <= batch <= 32767, 1 <= heads <= 65535, 1 <= rows < 2^31 - 64, dim a multiple of 16 up to "
+                "256, block 16, 32 or 64 (got %lld, %lld, %lld, %lld, %d)", who, static_cast<long long>(d->batch),
+                static_cast<long long>(d->heads), static_cast<long long>(d->rows), static_cast<long long>(d->dim),
+                d->block);
+        return false;
+    }
+    if (((reinterpret_cast<uintptr_t>(d->k) | reinterpret_cast<uintptr_t>(d->v)) & 15) ||
+        ((reinterpret_cast<uintptr_t>(d->k_scale) | reinterpret_cast<uintptr_t>(d->v_scale)) & 3) || d->bs % 16 ||
+        d->hs % 16 || d->rs % 16 || d->rs < d->dim || (d->heads > 1 && d->hs < d->dim) ||
+        (d->batch > 1 && d->bs < d->dim)) {
+        set_err("%s: codes must be 16-byte aligned with strides that are multiples of 16 and at least dim", who);
+        return false;
+    }
+    const int64_t nb = (d->rows + d->block - 1) / d->block;
+    if ((d->heads > 1 && d->shs < nb) || (d->batch > 1 && d->sbs < nb)) {
+        set_err("%s: the scales need strides of at least rows / block", who);
+        return false;
+    }
+    if (T < 0 || T > 0x7fffffff) {
+        set_err("%s: bad token count %lld", who, static_cast<long long>(T));
+        return false;
+    }
+    c = Kv8Cache{d->k, d->v, d->k_scale, d->v_scale, d->bs, d->hs, d->rs, d->sbs, d->shs,
+                 static_cast<int>(d->batch), static_cast<int>(d->heads), static_cast<int>(d->rows),
+                 static_cast<int>(d->dim), d->block == 16 ? 4 : d->block == 32 ? 5 : 6};
+    r = Kv8Rows{pos, cnt, static_cast<int>(T), nullptr};
+    return true;
+}
+// token rows of n values: aligned, and (several of them) at least n apart
+bool kv8_check_rows(const char *who, const char *name, const void *p, int64_t ld, int64_t n, int64_t rows, bool bf16) {
+    const int elt = bf16 ? 2 : 4;
+    if (!p || (reinterpret_cast<uintptr_t>(p) & 15) || (rows > 1 && (ld < n || ld * elt % 16))) {
+        set_err("%s: rows of %s must be 16-byte aligned with a stride of whole 16 bytes and at least %lld values", who,
+                name, static_cast<long long>(n));
+        return false;
+    }
+    return true;
+}
+// last: the device, whose status word a skipped sequence sets
+bool kv8_device(const char *who, Kv8Rows &r) {
+    Ctx &x = ctx();
+    if (!x.ok) {
+        set_err("no usable CUDA device");
+        return false;
+    }
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev != x.device) {
+        set_err("%s: the current device is %d, the library's is %d", who, dev, x.device);
+        return false;
+    }
+    r.err = x.d_err;
+    return true;
+}
+bool kv8_check_heads(const char *who, const onpu_kv8_cache *d, int Hq) {
+    if (Hq >= 1 && Hq % d->heads == 0 && Hq / d->heads <= 16) return true;
+    set_err("%s: need Hq %% heads == 0 with Hq / heads <= 16 (got Hq %d, heads %lld)", who, Hq,
+            static_cast<long long>(d->heads));
+    return false;
+}
+}  // namespace
+
+int onpu_kv8_append_dev(const onpu_kv8_cache *cache, const void *k, int64_t ldk, const void *v, int64_t ldv, int64_t T,
+                        int x_bf16, const int32_t *pos, const int32_t *cnt, void *stream) {
+    clear_err();
+    const char *who = "onpu_kv8_append_dev";
+    Kv8Cache c;
+    Kv8Rows r;
+    if (!kv8_check(who, cache, T, pos, cnt, c, r)) return -1;
+    if (T == 0) return 0;
+    const int64_t n = cache->heads * cache->dim, rows = cache->batch * T;
+    if (!kv8_check_rows(who, "k", k, ldk, n, rows, x_bf16) || !kv8_check_rows(who, "v", v, ldv, n, rows, x_bf16) ||
+        !kv8_device(who, r))
+        return -1;
+    ONPU_CUDA(kv8_append_launch(c, r, k, ldk, v, ldv, x_bf16 != 0, static_cast<cudaStream_t>(stream)), -1);
+    return 0;
+}
+
+int onpu_kv8_read_dev(const onpu_kv8_cache *cache, void *k, int64_t ldk, void *v, int64_t ldv, int64_t T, int x_bf16,
+                      const int32_t *pos, const int32_t *cnt, void *stream) {
+    clear_err();
+    const char *who = "onpu_kv8_read_dev";
+    Kv8Cache c;
+    Kv8Rows r;
+    if (!kv8_check(who, cache, T, pos, cnt, c, r)) return -1;
+    if (T == 0) return 0;
+    const int64_t n = cache->heads * cache->dim, rows = cache->batch * T;
+    if (!kv8_check_rows(who, "k", k, ldk, n, rows, x_bf16) || !kv8_check_rows(who, "v", v, ldv, n, rows, x_bf16) ||
+        !kv8_device(who, r))
+        return -1;
+    ONPU_CUDA(kv8_read_launch(c, r, k, ldk, v, ldv, x_bf16 != 0, static_cast<cudaStream_t>(stream)), -1);
+    return 0;
+}
+
+int64_t onpu_kv8_attn_ws(const onpu_kv8_cache *cache, int Hq, int64_t T, int x_bf16) {
+    clear_err();
+    const char *who = "onpu_kv8_attn_ws";
+    Kv8Cache c;
+    Kv8Rows r;
+    const int32_t none = 0;
+    if (!kv8_check(who, cache, T, &none, nullptr, c, r) || !kv8_check_heads(who, cache, Hq) ||
+        !kv8_device(who, r))
+        return -1;
+    return kv8_attn_ws_bytes(Hq, c.Hkv, c.D, r.T, x_bf16 != 0);
+}
+
+int onpu_kv8_attn_dev(const onpu_kv8_cache *cache, const void *q, int64_t ldq, int Hq, int64_t T, int x_bf16,
+                      const int32_t *pos, const int32_t *cnt, const float *mask, int64_t mask_bs, int64_t mask_ts,
+                      const float *sinks, float scale, void *out, int64_t ldo, void *ws, void *stream) {
+    clear_err();
+    const char *who = "onpu_kv8_attn_dev";
+    Kv8AttnParams p{};
+    if (!kv8_check(who, cache, T, pos, cnt, p.c, p.r) || !kv8_check_heads(who, cache, Hq)) return -1;
+    if (T == 0) return 0;
+    const int64_t n = Hq * cache->dim, rows = cache->batch * T;
+    if (!kv8_check_rows(who, "q", q, ldq, n, rows, x_bf16) || !kv8_check_rows(who, "out", out, ldo, n, rows, x_bf16))
+        return -1;
+    if (!ws || (reinterpret_cast<uintptr_t>(ws) & 15)) {
+        set_err("%s: ws must be 16-byte aligned device memory of onpu_kv8_attn_ws bytes", who);
+        return -1;
+    }
+    if (!kv8_device(who, p.r)) return -1;
+    p.q = q;
+    p.ldq = ldq;
+    p.out = out;
+    p.ldo = ldo;
+    p.Hq = Hq;
+    p.mask = mask;
+    p.mbs = mask_bs;
+    p.mts = mask_ts;
+    p.sinks = sinks;
+    p.scale = scale;
+    p.ws = ws;
+    ONPU_CUDA(kv8_attn_launch(p, x_bf16 != 0, static_cast<cudaStream_t>(stream)), -1);
+    return 0;
 }
 
 int onpu_layout_version(void) { return kGpuLayoutVersion; }

@@ -79,6 +79,10 @@ SIGNATURES = {
     "onpu_dense_mm_dev": (I32, [P, P, I64, I64, P, I64, I32, P]),
     "onpu_dense_unpack_dev": (I32, [P, P, P, P, P]),
     "onpu_attn_step_dev": (I32, [P, I32, I32, P, P, I32, I64, I64, I64, P, P, C.c_float, P, I32, P]),
+    "onpu_kv8_append_dev": (I32, [P, P, I64, P, I64, I64, I32, P, P, P]),
+    "onpu_kv8_read_dev": (I32, [P, P, I64, P, I64, I64, I32, P, P, P]),
+    "onpu_kv8_attn_dev": (I32, [P, P, I64, I32, I64, I32, P, P, P, I64, I64, P, C.c_float, P, I64, P, P]),
+    "onpu_kv8_attn_ws": (I64, [P, I32, I64, I32]),
     "onpu_layout_version": (I32, []),
     "onpu_dense_export": (I64, [P, P, I64]),
     "onpu_dense_import": (P, [P, I64]),
@@ -211,3 +215,11 @@ class GgmlTensor(C.Structure):
 
 GGML_OP_VIEW, GGML_OP_MUL_MAT, GGML_OP_MUL_MAT_ID = 0, 1, 2
 GGML_F32, GGML_F16, GGML_Q4_0, GGML_Q4_K, GGML_I32, GGML_BF16 = 0, 1, 2, 12, 26, 30
+
+
+class Kv8Cache(C.Structure):
+    """onpu_kv8_cache: where an 8-bit KV cache lies (include/onpu.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("batch", C.c_int64), ("heads", C.c_int64), ("rows", C.c_int64), ("dim", C.c_int64),
+                ("bs", C.c_int64), ("hs", C.c_int64), ("rs", C.c_int64), ("sbs", C.c_int64), ("shs", C.c_int64),
+                ("block", C.c_int32)]

@@ -477,3 +477,61 @@ def attn_step_ref(L, q, K, V, mask=None, sinks=None, scale=None, bf16=False):
     f(fp(q), Hq, D, K.ctypes.data, V.ctypes.data, Hkv, S, S * D, D, fp(m), fp(sk),
       float(D ** -0.5 if scale is None else scale), fp(out))
     return out
+
+
+# ---------------------------------------------------------------- the 8-bit KV cache (no reference counterpart)
+def kv8_append(codes, scales, x, pos, cnt, block):
+    """Quantise rows x [B, T, H, D] into codes (int8 [B, H, S, D]) and scales (fp32 [B, H, nblocks]) in
+    place, in float64: token i < cnt[b] of sequence b is row pos[b] + i. Blocks that hold a new row:
+    scale = max(old scale, fl32(largest new |value| / 127)), old = 0 where the block holds no earlier
+    row; codes = rint(value / scale); earlier rows of a block whose scale grew are re-rounded onto it. A
+    value that is not finite makes the block's scale NaN, its new codes 0."""
+    for b in range(codes.shape[0]):
+        p, end = int(pos[b]), int(pos[b]) + int(cnt[b])
+        for h in range(codes.shape[1]):
+            for i in range(p // block, (end - 1) // block + 1 if end > p else p // block):
+                lo, hi = max(p, i * block), min(end, (i + 1) * block)
+                v = x[b, lo - p:hi - p, h].astype(np.float64)
+                old = np.float32(scales[b, h, i] if lo > i * block else 0)
+                if not np.isfinite(v).all() or np.isnan(old):
+                    scales[b, h, i] = np.nan
+                    codes[b, h, lo:hi] = 0
+                    continue
+                new = max(old, np.float32(np.abs(v).max() / 127.0))
+                if new > old and lo > i * block:
+                    c = codes[b, h, i * block:lo].astype(np.float64)
+                    codes[b, h, i * block:lo] = np.rint(c * np.float64(old) / np.float64(new))
+                codes[b, h, lo:hi] = np.clip(np.rint(v / np.float64(new)), -127, 127) if new > 0 else 0
+                scales[b, h, i] = new
+
+
+def kv8_values(codes, scales, block):
+    """code * scale in float64, [B, H, S, D]."""
+    s = np.repeat(scales.astype(np.float64), block, axis=2)[:, :, :codes.shape[2], None]
+    return codes.astype(np.float64) * s
+
+
+def kv8_attn(q, K, V, pos, cnt, mask=None, sinks=None, scale=None):
+    """q [B, T, Hq, D], K and V float64 [B, H, S, D] -> float64 [B, T, Hq, D] and the bound sums
+    sum |q_d K_jd| * scale (its largest over the rows seen) [B, T, Hq]: query i sees rows 0 .. pos + i
+    whose mask [B, T, S] is not -inf; zeros where none is left, and for i >= cnt."""
+    B, T, Hq, D = q.shape
+    rep = Hq // K.shape[1]
+    scale = D ** -0.5 if scale is None else scale
+    out, big = np.zeros((B, T, Hq, D)), np.zeros((B, T, Hq))
+    for b in range(B):
+        for i in range(int(cnt[b])):
+            rows = np.arange(int(pos[b]) + i + 1)
+            m = np.zeros(len(rows)) if mask is None else mask[b, i, :len(rows)].astype(np.float64)
+            rows, m = rows[~np.isneginf(m)], m[~np.isneginf(m)]
+            if not len(rows):
+                continue
+            for h in range(Hq):
+                qv, Kv, Vv = q[b, i, h].astype(np.float64), K[b, h // rep, rows], V[b, h // rep, rows]
+                x = Kv @ qv * scale + m
+                top = max(x.max(), -np.inf if sinks is None else float(sinks[h]))
+                e = np.exp(x - top)
+                total = e.sum() + (0.0 if sinks is None else np.exp(float(sinks[h]) - top))
+                out[b, i, h] = e @ Vv / total
+                big[b, i, h] = (np.abs(Kv) @ np.abs(qv)).max() * abs(scale)
+    return out, big
