@@ -29,13 +29,13 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
-#include <cudaTypedefs.h>
 
 #include <cstdio>
 
 #include "gpu_layout.cuh"
 #include "kernels.h"
 #include "ptx.cuh"
+#include "tmap.h"
 
 namespace onpu_b200 {
 
@@ -501,20 +501,6 @@ cudaError_t launch_fmt(int epi, const CUtensorMap &map, const DqGemmParams &p, c
     }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static bool tried = false;
-    if (!tried) {
-        tried = true;
-        void *ptr = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-    }
-    return fn;
-}
-
 }  // namespace
 
 int dqgemm_tile_tokens() { return kTM; }
@@ -527,7 +513,7 @@ cudaError_t x_to_f16_launch(const uint16_t *x, int64_t ldx, int M, int K, uint16
 }
 
 cudaError_t dqgemm_launch(int fmt, int epi, const uint16_t *xh, const DqGemmParams &p, cudaStream_t stream) {
-    auto fn = encode_fn();
+    auto fn = tensor_map_encode_fn();
     if (!fn) return cudaErrorNotSupported;
     CUtensorMap map;
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.K), static_cast<cuuint64_t>(p.M)};

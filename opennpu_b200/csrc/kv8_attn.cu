@@ -34,11 +34,13 @@
 #include "kernels.h"
 #include "kv8.cuh"
 #include "ptx.cuh"
+#include "tmap.h"
 
 namespace onpu_b200 {
 namespace {
 
-constexpr int kWarps = 4, kStep = 16, kUnit = kWarps * kStep;
+constexpr int kWarps = 4;
+constexpr uint64_t kWaitNs = 2000000000ull;   // bound of every wait for a copy
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -84,27 +86,28 @@ __device__ __forceinline__ float pow2_to(float x, int top) {
     if (e == 255 || !(fabsf(x) > 0.f)) return 1.f;
     return __uint_as_float(static_cast<uint32_t>(127 + min(100, max(-100, top + 127 - e))) << 23);
 }
-__device__ __forceinline__ void cp_async_4(uint32_t dst, const void *src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ float max_nan(float a, float b) {     // NaN where either is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // ---------------------------------------------------------------- the list of units
-// An entry is a (sequence, query tile); its rows are counted in 64-row units, once per kv head.
+// An entry is a (sequence, query tile); its rows are counted in units of kWarps * 16 R, once per kv head.
 struct Plan {
-    int rep, tile, tiles, entries;    // query heads per kv head, queries a tile, tiles a sequence, B * tiles
-    __device__ __forceinline__ Plan(const Kv8AttnParams &p, int tile_) {
+    int rep, tile, tiles, entries, unit;    // query heads per kv head, queries a tile, tiles a sequence, B * tiles
+    __device__ __forceinline__ Plan(const Kv8AttnParams &p, int tile_, int unit_) {
         rep = p.Hq / p.c.Hkv;
         tile = tile_;
+        unit = unit_;
         tiles = static_cast<int>((static_cast<int64_t>(p.r.T) * rep + tile - 1) / tile);
         entries = p.c.B * tiles;
     }
     // rows that entry e's tile sees (0: nothing of it is valid)
     __device__ __forceinline__ int rows(const Kv8AttnParams &p, int e, int &pos, int &cnt) const {
-        const int b = e / tiles;
+        const int b = tiles == 1 ? e : e / tiles;
         if (!kv8_rows(p.r, b, p.c.S, pos, cnt)) return 0;
+        if (tiles == 1) return cnt > 0 ? pos + cnt : 0;
         const int64_t r0 = static_cast<int64_t>(e - b * tiles) * tile;
         const int first = static_cast<int>(r0 / rep), last = static_cast<int>((r0 + tile - 1) / rep);
         if (first >= cnt) return 0;
@@ -112,7 +115,8 @@ struct Plan {
     }
     __device__ __forceinline__ int units(const Kv8AttnParams &p, int e) const {
         int pos, cnt;
-        return static_cast<int>((static_cast<int64_t>(rows(p, e, pos, cnt)) + kUnit - 1) / kUnit);
+        const unsigned n = rows(p, e, pos, cnt);
+        return static_cast<int>((n + unit - 1) / unit);
     }
 };
 __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
@@ -120,15 +124,17 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// units of all entries and heads (every lane of the warp gets it)
-__device__ __forceinline__ int64_t total_units(const Kv8AttnParams &p, const Plan &pl, int lane) {
-    int64_t n = 0;
-    for (int e = lane; e < pl.entries; e += 32) n += pl.units(p, e);
-    return warp_sum64(n) * p.c.Hkv;
+// a / b, in 32 bits where they fit (they all but always do; a 64-bit division costs a few hundred instructions)
+__device__ __forceinline__ int64_t div64(int64_t a, int64_t b) {
+    if (((a | b) >> 31) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
 }
-// CTA i of W takes units [cta_first(i), cta_first(i + 1)), at least one each: W = min(grid, N)
-__device__ __forceinline__ int64_t cta_first(int64_t N, int cta, int W) { return N * cta / W; }
-__device__ __forceinline__ int cta_of(int64_t N, int64_t u, int W) { return static_cast<int>(((u + 1) * W - 1) / N); }
+// units a CTA takes: N units over G CTAs, at least kMinUnits each (a part shorter than that costs more to
+// join than it saves); CTA i has units [i * per, (i + 1) * per) of the list
+constexpr int kMinUnits = 1;
+__device__ __forceinline__ int64_t units_per_cta(int64_t N, int G) {
+    return max(static_cast<int64_t>(kMinUnits), div64(N + G - 1, G));
+}
 
 // ws: per CTA two slots of [tile][DP] outputs, then per slot [tile] (reference, sum) pairs
 template <int DP>
@@ -167,43 +173,72 @@ __device__ __forceinline__ float out_factor(float M, float Lsum, const float *si
 }
 
 // ---------------------------------------------------------------- the split kernel
-template <int DP>
-constexpr int kStageBytes = 2 * kStep * DP + 16;              // 16 rows of K and V, their two scales
+// A stage: 16 R rows of K, then of V, as TMA wrote them: rows of 64 or 128 bytes (256: two such halves one
+// after the other), their 16-byte chunks exchanged by the map's swizzle.
+template <int DP, int R>
+constexpr int kStageBytes = 2 * 16 * R * DP;
 template <int DP, int NT>
 constexpr int kMergeBytes = kWarps * 8 * NT * ((DP + 4) * 4 + 8);
 
-// byte offset of 16-byte chunk c of row r (of 16) in a staged tile: chunks are exchanged so that neither the
-// eight-lane phases of the K reads (rows r, r + 1, four chunks) nor those of the V reads (rows 4 apart, one
-// or two chunks) meet in a bank
+// byte offset of chunk c of row r in a tile of `rows` rows
 template <int DP>
-__device__ __forceinline__ int stage_off(int r, int c) {
-    if constexpr (DP == 64) return r * DP + ((c ^ (r >> 2 & 3)) << 4);
-    else return r * DP + ((c ^ (((r ^ (r >> 3)) & 1) << 2 | (r >> 2 & 1) << 1)) << 4);
+__device__ __forceinline__ int stage_off(int rows, int r, int c) {
+    if constexpr (DP == 64) return r * 64 + ((c ^ (r >> 1 & 3)) << 4);
+    else return (c >> 3) * rows * 128 + r * 128 + (((c ^ r) & 7) << 4);
+}
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap *map, int x, int row, int head, int seq,
+                                         uint32_t bar, uint64_t pol) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, "
+        "%4, %5}], [%6], %7;" ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(head), "r"(seq), "r"(bar), "l"(pol)
+        : "memory");
+}
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8u8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int DP, int NT, bool BF16, bool MASK, int NS>
-__global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const Kv8AttnParams p) {
-    constexpr int PARTS = BF16 ? 1 : 2;
+template <int DP, int NT, bool BF16, bool MASK, int R, int NS>
+__global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __grid_constant__ CUtensorMap mapk,
+                                                                     const __grid_constant__ CUtensorMap mapv,
+                                                                     const Kv8AttnParams p) {
+    constexpr int PARTS = BF16 ? 1 : 2;             // fp16 parts of a weight
     constexpr int KI = DP / 64;                     // 16-byte chunks of a K row per lane
     constexpr int VW = DP / 32;                     // 4-byte words of a V row per lane
-    constexpr int CH = DP / 16;                     // chunks per row
-    constexpr int STB = kStageBytes<DP>;
+    constexpr int ROWS = 16 * R, STB = kStageBytes<DP, R>;
     constexpr float U = MASK ? kLog2e : 1.f, RAISE = MASK ? 4.f : 6.f;
-    extern __shared__ __align__(128) uint8_t smem[];
-    pdl_launch_dependents();
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[kWarps * NS];
+    uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);      // the swizzle's period
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int G = gridDim.x, D = p.c.D, nch = D >> 4;
+    const int G = gridDim.x, D = p.c.D;
     const Kv8Cache &c = p.c;
-    uint8_t *wbuf = smem + warp * NS * STB;
-    const uint32_t wbase = smem_u32(wbuf);
+    const uint32_t wbase = smem_u32(smem) + warp * NS * STB, bar0 = smem_u32(bars) + warp * NS * 8;
+    if (lane == 0) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) mbar_init(bar0 + 8 * s, 1);
+        mbar_init_fence();
+    }
+    const uint64_t pol = l2_evict_first_policy();
+    __syncwarp();
     pdl_wait_prerequisites();
+    pdl_launch_dependents();              // after the wait: the join may read pos and cnt as it starts
 
-    const Plan pl(p, 8 * NT);
-    const int64_t N = total_units(p, pl, lane);
-    const int W = static_cast<int>(min(N, static_cast<int64_t>(G)));
-    if (static_cast<int>(blockIdx.x) >= W) return;
-    int64_t u = cta_first(N, blockIdx.x, W);
-    const int64_t u1 = cta_first(N, blockIdx.x + 1, W);
+    const Plan pl(p, 8 * NT, kWarps * ROWS);
+    // units of all entries and heads
+    int64_t N = 0;
+    for (int e = lane; e < pl.entries; e += 32) N += pl.units(p, e);
+    N = warp_sum64(N) * c.Hkv;
+    const int64_t per = units_per_cta(N, G);
+    int64_t u = per * blockIdx.x;
+    const int64_t u1 = min(N, u + per);
+    if (u >= u1) return;
     // the entry that holds unit u, and its first unit
     int e = 0, n = 0;
     int64_t e0 = 0;
@@ -226,47 +261,60 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const Kv8At
         e0 += __shfl_sync(0xffffffffu, incl, 31);
     }
 
-    bool first_seg = true;
-    const int ra = 4 * (g >> 1) + (g & 1), rb = ra + 2;       // this lane's K rows of a step
+    bool first_seg = true, failed = false;
+    int stage = 0, filled = 0;                     // the next stage to read and its parity, the next to fill
+    uint32_t parity = 0;
+    // this lane's rows of a 16-row block: for V (4 of them) and, of those that lanes 4 (g / 2) .. hold, for K
+    // (two). Rows 2p and (2p ^ 4) + 1 [+ 8]: in the swizzled tile the eight lanes of a phase never meet in a bank.
+    const int vr0 = 2 * t, vr1 = ((2 * t) ^ 4) + 1;
+    const int kp = g >> 1, ra = g & 1 ? ((2 * kp) ^ 4) + 1 : 2 * kp, rb = ra + 8;
     while (u < u1) {
         while (n == 0 || u >= e0 + static_cast<int64_t>(n) * c.Hkv) {     // the next entry with rows
             e0 += static_cast<int64_t>(n) * c.Hkv;
             n = pl.units(p, ++e);
         }
-        const int h = static_cast<int>((u - e0) / n), ua = static_cast<int>(u - e0 - static_cast<int64_t>(h) * n);
+        const int h = static_cast<int>(div64(u - e0, n)), ua = static_cast<int>(u - e0 - static_cast<int64_t>(h) * n);
         const int ub = static_cast<int>(min(static_cast<int64_t>(n), ua + (u1 - u)));
         int pos, cnt;
-        const int len = pl.rows(p, e, pos, cnt), b = e / pl.tiles;
+        const int len = pl.rows(p, e, pos, cnt), b = pl.tiles == 1 ? e : e / pl.tiles;
         const int64_t q0 = static_cast<int64_t>(e - b * pl.tiles) * pl.tile;         // the tile's first query
         const int nq = static_cast<int>(min(static_cast<int64_t>(pl.tile), static_cast<int64_t>(cnt) * pl.rep - q0));
-        const int row0 = ua * kUnit, row1 = static_cast<int>(min(static_cast<int64_t>(len), static_cast<int64_t>(ub) * kUnit));
-        const int nstep = (row1 - row0 + kStep - 1) / kStep;
-        const int8_t *Kb = c.k + b * c.bs + h * c.hs, *Vb = c.v + b * c.bs + h * c.hs;
+        const int row0 = ua * kWarps * ROWS;
+        const int row1 = static_cast<int>(min(static_cast<int64_t>(len), static_cast<int64_t>(ub) * kWarps * ROWS));
+        const int nstep = (row1 - row0 + ROWS - 1) / ROWS;
         const float *ksb = c.ks + b * c.sbs + h * c.shs, *vsb = c.vs + b * c.sbs + h * c.shs;
 
-        auto issue = [&](int s, int stage) {                    // step s (every kWarps-th is this warp's) into a stage
-            if (s < nstep) {
-                const int r0 = row0 + s * kStep;
-                const uint32_t st = wbase + stage * STB;
+        auto issue = [&](int s) {                  // step s (every kWarps-th is this warp's) into the next stage
+            if (s < nstep && !failed) {
+                if (lane == 0) {
+                    const uint32_t st = wbase + filled * STB, bar = bar0 + 8 * filled;
+                    const int r0 = row0 + s * ROWS;
+                    mbar_arrive_expect_tx(bar, STB);
 #pragma unroll
-                for (int i = 0; i < kStep * CH / 32; ++i) {
-                    const int idx = lane + 32 * i, r = idx / CH, ch = idx % CH;
-                    if (r0 + r < row1 && ch < nch) {
-                        const int64_t go = static_cast<int64_t>(r0 + r) * c.rs + ch * 16;
-                        const int so = stage_off<DP>(r, ch);
-                        cp_async_16(st + so, Kb + go, 16);
-                        cp_async_16(st + kStep * DP + so, Vb + go, 16);
+                    for (int x = 0; x < DP; x += 128) {
+                        tma_rows(st + x * ROWS, &mapk, x, r0, h, b, bar, pol);
+                        tma_rows(st + DP * ROWS + x * ROWS, &mapv, x, r0, h, b, bar, pol);
                     }
                 }
-                if (lane < 2) cp_async_4(st + 2 * kStep * DP + 4 * lane, (lane ? vsb : ksb) + (r0 >> c.blk_log2));
+                filled = filled + 1 == NS ? 0 : filled + 1;
             }
-            cp_commit();
         };
 #pragma unroll
-        for (int s = 0; s < NS - 1; ++s) issue(warp + s * kWarps, s);
+        for (int s = 0; s < NS - 1; ++s) issue(warp + s * kWarps);
+        float ksc[R], vsc[R];                      // the scales of this warp's next step
+        auto load_scales = [&](int s) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int r = row0 + s * ROWS + 16 * i;
+                ksc[i] = r < row1 ? ksb[r >> c.blk_log2] : 0.f;
+                vsc[i] = r < row1 ? vsb[r >> c.blk_log2] : 0.f;
+            }
+        };
+        load_scales(warp);
 
-        // q^T as B fragments: k slots (2t, 2t+1 | 2t+8, 2t+9) of step (i, w) are d = 16 (t + 4i) + 4w + (0, 1 | 2, 3)
-        uint32_t qf[PARTS][NT][KI * 4][2];
+        // q^T as B fragments of base-256 digits: q f = 2^16 d0 + 2^8 d1 + d2, d0 signed, f the power of two that puts
+        // the row's largest |q f| in [2^22, 2^23). Lane t's k slots of step (i, s) are d = 16 (t + 4i) + 8s + 0 .. 7.
+        uint32_t qf[3][NT][KI * 2][2];
         float rs[NT][2];
         int lim[NT][2];
         int64_t moff[NT][2];
@@ -274,7 +322,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const Kv8At
         for (int nt = 0; nt < NT; ++nt) {
             const int qi = 8 * nt + g;
             const bool ok = qi < nq;
-            const int tok = static_cast<int>((q0 + (ok ? qi : 0)) / pl.rep);
+            const int tok = static_cast<int>(div64(q0 + (ok ? qi : 0), pl.rep));
             const int hq = h * pl.rep + static_cast<int>((q0 + (ok ? qi : 0)) - static_cast<int64_t>(tok) * pl.rep);
             const int64_t qo = (static_cast<int64_t>(b) * p.r.T + tok) * p.ldq + static_cast<int64_t>(hq) * D;
             float x[KI * 4][4];
@@ -299,24 +347,25 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const Kv8At
                     x[i * 4 + w][2] = v.z;
                     x[i * 4 + w][3] = v.w;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) mx = fmaxf(mx, fabsf(x[i * 4 + w][k]));
+                    for (int k = 0; k < 4; ++k) mx = max_nan(mx, fabsf(x[i * 4 + w][k]));
                 }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float f = pow2_to(mx, 8);
+            mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float f = pow2_to(mx, 22);
 #pragma unroll
-            for (int s = 0; s < KI * 4; ++s)
+            for (int s = 0; s < KI * 4; ++s) {
+                uint32_t dg[3] = {0, 0, 0};
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const float v0 = x[s][2 * k] * f, v1 = x[s][2 * k + 1] * f;
-                    qf[0][nt][s][k] = pack_h2(v0, v1);
-                    if constexpr (PARTS == 2) {
-                        const float2 r = unpack_h2(qf[0][nt][s][k]);
-                        qf[PARTS - 1][nt][s][k] = pack_h2(v0 - r.x, v1 - r.y);
-                    }
+                for (int k = 0; k < 4; ++k) {
+                    const int Q = __float2int_rn(x[s][k] * f);
+#pragma unroll
+                    for (int j = 0; j < 3; ++j) dg[j] |= static_cast<uint32_t>(Q >> (16 - 8 * j) & 0xff) << (8 * k);
                 }
-            // what a lane's columns 2t, 2t + 1 of the scores need
-            const float rsg = p.scale * (MASK ? 1.f : kLog2e) / f;
+#pragma unroll
+                for (int j = 0; j < 3; ++j) qf[j][nt][s >> 1][s & 1] = dg[j];
+            }
+            // what a lane's columns 2t, 2t + 1 of the scores need; a query that is not finite has NaN scores
+            const float rsg = mx < INFINITY ? p.scale * (MASK ? 1.f : kLog2e) / f : __uint_as_float(0x7fc00000u);
             const int lg = ok ? pos + tok : -1;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -326,7 +375,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const Kv8At
             }
         }
         // the first row that some query of the tile must not see (queries past nq do not matter)
-        const int edge = pos + static_cast<int>(q0 / pl.rep) + 1;
+        const int edge = pos + static_cast<int>(div64(q0, pl.rep)) + 1;
 
         float o[VW * 2][NT][4], m[NT][2], l[NT][2], cv = 0.f;
 #pragma unroll
@@ -336,81 +385,94 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const Kv8At
             m[nt][0] = m[nt][1] = -INFINITY;
             l[nt][0] = l[nt][1] = 0.f;
         }
-        float mk[NT][4];                                       // the mask of this warp's next step
+        float mk[R][NT][4];                                    // the mask of this warp's next step
         auto load_mask = [&](int s) {
             if constexpr (MASK) {
-                const int ja = row0 + s * kStep + ra;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int i = 0; i < R; ++i)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int j = ja + (k & 2);
-                        mk[nt][k] = s < nstep && j <= lim[nt][k & 1] ? p.mask[moff[nt][k & 1] + j] : -INFINITY;
-                    }
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int j = row0 + s * ROWS + 16 * i + (k & 2 ? rb : ra);
+                            mk[i][nt][k] = s < nstep && j <= lim[nt][k & 1] ? p.mask[moff[nt][k & 1] + j] : -INFINITY;
+                        }
             }
         };
         load_mask(warp);
-        int stage = 0;
         for (int s = warp; s < nstep; s += kWarps) {
             __syncwarp();                                      // every lane is past its reads of the stage refilled here
-            issue(s + (NS - 1) * kWarps, stage == 0 ? NS - 1 : stage - 1);
-            cp_wait<NS - 1>();
-            __syncwarp();
-            const uint32_t kb = wbase + stage * STB, vb = kb + kStep * DP;
+            issue(s + (NS - 1) * kWarps);
+            if (!failed) failed = __any_sync(0xffffffffu, !mbar_wait_bounded(bar0 + 8 * stage, parity, kWaitNs));
+            const uint32_t kb = wbase + stage * STB, vb = kb + DP * ROWS;
             stage = stage + 1 == NS ? 0 : stage + 1;
-            const float2 ksv = *reinterpret_cast<const float2 *>(smem + (vb + kStep * DP - smem_u32(smem)));
-            const int r0 = row0 + s * kStep;
-            float x[NT][4];
-            {
-                float acc[NT][2][4];                           // two chains a tile
+            parity ^= stage == 0;
+            const int r0 = row0 + s * ROWS;
+            float x[R][NT][4], sv[R];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+            for (int i = 0; i < R; ++i) {
+                int acc[3][NT][4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[nt][0][k] = acc[nt][1][k] = 0.f;
+                for (int j = 0; j < 3; ++j)
 #pragma unroll
-                for (int i = 0; i < KI; ++i) {
-                    const uint4 va = lds_v4(kb + stage_off<DP>(ra, t + 4 * i)), vv = lds_v4(kb + stage_off<DP>(rb, t + 4 * i));
-                    const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vv.x, vv.y, vv.z, vv.w};
+                    for (int nt = 0; nt < NT; ++nt) acc[j][nt][0] = acc[j][nt][1] = acc[j][nt][2] = acc[j][nt][3] = 0;
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint32_t xa = wa[w] ^ 0x80808080u, xb = wb[w] ^ 0x80808080u;
-                        const uint32_t a0 = h2_lo(xa), a1 = h2_lo(xb), a2 = h2_hi(xa), a3 = h2_hi(xb);
+                for (int k = 0; k < KI; ++k) {
+                    const uint4 va = lds_v4(kb + stage_off<DP>(ROWS, 16 * i + ra, t + 4 * k));
+                    const uint4 vv = lds_v4(kb + stage_off<DP>(ROWS, 16 * i + rb, t + 4 * k));
+                    const uint32_t a[2][4] = {{va.x, vv.x, va.y, vv.y}, {va.z, vv.z, va.w, vv.w}};
 #pragma unroll
-                        for (int pt = 0; pt < PARTS; ++pt)
+                    for (int w = 0; w < 2; ++w)
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-                                mma_f16(acc[nt][w & 1], a0, a1, a2, a3, qf[pt][nt][i * 4 + w][0], qf[pt][nt][i * 4 + w][1]);
-                    }
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma_s8(acc[0][nt], a[w], qf[0][nt][k * 2 + w][0], qf[0][nt][k * 2 + w][1]);
+                            mma_s8u8(acc[1][nt], a[w], qf[1][nt][k * 2 + w][0], qf[1][nt][k * 2 + w][1]);
+                            mma_s8u8(acc[2][nt], a[w], qf[2][nt][k * 2 + w][0], qf[2][nt][k * 2 + w][1]);
+                        }
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const float f0 = ksv.x * rs[nt][0], f1 = ksv.x * rs[nt][1];
+                    const float f[2] = {ksc[i] * rs[nt][0], ksc[i] * rs[nt][1]};
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        x[nt][k] = (acc[nt][0][k] + acc[nt][1][k]) * (k & 1 ? f1 : f0);
-                        if constexpr (MASK) x[nt][k] = mk[nt][k] == -INFINITY ? -INFINITY : x[nt][k] + mk[nt][k];
+                    for (int k = 0; k < 4; ++k) {              // |acc[0] 2^8 + acc[1]| < 2^31
+                        const float a = fmaf(static_cast<float>(acc[0][nt][k] * 256 + acc[1][nt][k]), 256.f,
+                                             static_cast<float>(acc[2][nt][k]));
+                        x[i][nt][k] = a * f[k & 1];
+                        if constexpr (MASK)
+                            x[i][nt][k] = mk[i][nt][k] == -INFINITY ? -INFINITY : x[i][nt][k] + mk[i][nt][k];
                     }
                 }
+                sv[i] = vsc[i];
             }
+            load_scales(s + kWarps);
             load_mask(s + kWarps);
-            if (!MASK && r0 + kStep > edge) {                  // MASK: load_mask gave -inf beyond the limits
+            if (!MASK && r0 + ROWS > edge) {                   // MASK: load_mask gave -inf beyond the limits
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int i = 0; i < R; ++i)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (r0 + (k & 2 ? rb : ra) > lim[nt][k & 1]) x[nt][k] = -INFINITY;
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (r0 + 16 * i + (k & 2 ? rb : ra) > lim[nt][k & 1]) x[i][nt][k] = -INFINITY;
             }
             bool up = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) up |= x[nt][k] > m[nt][k & 1] + RAISE;
+                for (int k = 0; k < 2; ++k) {
+                    float mx = fmaxf(x[0][nt][k], x[0][nt][k + 2]);
+#pragma unroll
+                    for (int i = 1; i < R; ++i) mx = fmaxf(mx, fmaxf(x[i][nt][k], x[i][nt][k + 2]));
+                    up |= mx > m[nt][k] + RAISE;
+                }
             if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        float mx = fmaxf(x[nt][k], x[nt][k + 2]);
+                        float mx = fmaxf(x[0][nt][k], x[0][nt][k + 2]);
+#pragma unroll
+                        for (int i = 1; i < R; ++i) mx = fmaxf(mx, fmaxf(x[i][nt][k], x[i][nt][k + 2]));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -425,8 +487,11 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const Kv8At
                         }
                     }
             }
-            if (ksv.y * cv > 512.f || (cv == 0.f && ksv.y > 0.f)) {         // uniform: the weights' power of two
-                const float cn = pow2_to(ksv.y, 7), a = cv == 0.f ? 1.f : cn / cv;
+            float svm = sv[0];
+#pragma unroll
+            for (int i = 1; i < R; ++i) svm = fmaxf(svm, sv[i]);
+            if (svm * cv > 512.f || (cv == 0.f && svm > 0.f)) {             // uniform: the weights' power of two
+                const float cn = pow2_to(svm, 7), a = cv == 0.f ? 1.f : cn / cv;
                 cv = cn;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -435,69 +500,80 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const Kv8At
 #pragma unroll
                         for (int k = 0; k < 4; ++k) o[i][nt][k] *= a;
             }
-            const float sv = ksv.y * cv;
-            uint32_t pb[PARTS][NT][2];
+            uint32_t pb[R][PARTS][NT][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float w[4];
+            for (int i = 0; i < R; ++i) {
+                const float svc = sv[i] * cv;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float mr = m[nt][k & 1] == -INFINITY ? 0.f : m[nt][k & 1];
-                    const float e2 = ex2((x[nt][k] - mr) * U);
-                    l[nt][k & 1] += e2;
-                    w[k] = e2 * sv;
-                    // a row that is not seen weighs nothing, even where its scale is NaN
-                    if (x[nt][k] == -INFINITY) w[k] = 0.f;
-                }
+                for (int nt = 0; nt < NT; ++nt) {
+                    float w[4];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t hi = pack_h2(w[2 * k], w[2 * k + 1]);
-                    pb[0][nt][k] = movmatrix_trans(hi);
-                    if constexpr (PARTS == 2) {
-                        const float2 r = unpack_h2(hi);
-                        pb[PARTS - 1][nt][k] = movmatrix_trans(pack_h2(w[2 * k] - r.x, w[2 * k + 1] - r.y));
+                    for (int k = 0; k < 4; ++k) {
+                        const float mr = m[nt][k & 1] == -INFINITY ? 0.f : m[nt][k & 1];
+                        const float e2 = ex2((x[i][nt][k] - mr) * U);
+                        l[nt][k & 1] += e2;
+                        w[k] = e2 * svc;
+                        // a row that is not seen weighs nothing, even where its scale is NaN
+                        if (x[i][nt][k] == -INFINITY) w[k] = 0.f;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t hi = pack_h2(w[2 * k], w[2 * k + 1]);
+                        pb[i][0][nt][k] = movmatrix_trans(hi);
+                        if constexpr (PARTS == 2) {
+                            const float2 r = unpack_h2(hi);
+                            pb[i][PARTS - 1][nt][k] = movmatrix_trans(pack_h2(w[2 * k] - r.x, w[2 * k + 1] - r.y));
+                        }
                     }
                 }
             }
-            // V: words of rows 4t .. 4t + 3
+            // V: this lane's words of its four rows, MMA rows (2t, 2t + 1 | 2t + 8, 2t + 9) of the weights
 #pragma unroll
-            for (int v = 0; v < (DP == 256 ? 2 : 1); ++v) {
-                uint32_t wd[4][DP == 64 ? 2 : 4];
+            for (int i = 0; i < R; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if constexpr (DP == 64) {
-                        const uint2 q2 = lds_v2(vb + stage_off<DP>(4 * t + r, g >> 1) + (g & 1) * 8);
-                        wd[r][0] = q2.x;
-                        wd[r][1] = q2.y;
-                    } else {
-                        const uint4 q4 = lds_v4(vb + stage_off<DP>(4 * t + r, g + 8 * v));
-                        wd[r][0] = q4.x;
-                        wd[r][1] = q4.y;
-                        wd[r][2] = q4.z;
-                        wd[r][3] = q4.w;
+                for (int v = 0; v < (DP == 256 ? 2 : 1); ++v) {
+                    uint32_t wd[4][DP == 64 ? 2 : 4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int row = 16 * i + (r & 1 ? vr1 : vr0) + (r & 2 ? 8 : 0);
+                        if constexpr (DP == 64) {
+                            const uint2 q2 = lds_v2(vb + stage_off<DP>(ROWS, row, g >> 1) + (g & 1) * 8);
+                            wd[r][0] = q2.x;
+                            wd[r][1] = q2.y;
+                        } else {
+                            const uint4 q4 = lds_v4(vb + stage_off<DP>(ROWS, row, g + 8 * v));
+                            wd[r][0] = q4.x;
+                            wd[r][1] = q4.y;
+                            wd[r][2] = q4.z;
+                            wd[r][3] = q4.w;
+                        }
+                    }
+#pragma unroll
+                    for (int w = 0; w < (DP == 64 ? 2 : 4); ++w) {
+                        uint32_t y[4];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) y[r] = wd[r][w] ^ 0x80808080u;
+#pragma unroll
+                        for (int hf = 0; hf < 2; ++hf) {       // d = 4w + 2 hf + (0, 1)
+                            const uint32_t r01 = prmt(y[0], y[1], hf ? 0x7362u : 0x5140u);
+                            const uint32_t r23 = prmt(y[2], y[3], hf ? 0x7362u : 0x5140u);
+                            const uint32_t a0 = h2_lo(r01), a1 = h2_hi(r01), a2 = h2_lo(r23), a3 = h2_hi(r23);
+#pragma unroll
+                            for (int pt = 0; pt < PARTS; ++pt)
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt)
+                                    mma_f16(o[(v * 4 + w) * 2 + hf][nt], a0, a1, a2, a3, pb[i][pt][nt][0],
+                                            pb[i][pt][nt][1]);
+                        }
                     }
                 }
-#pragma unroll
-                for (int w = 0; w < (DP == 64 ? 2 : 4); ++w) {
-                    uint32_t y[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) y[r] = wd[r][w] ^ 0x80808080u;
-#pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {           // d = 4w + 2 hf + (0, 1)
-                        const uint32_t r01 = prmt(y[0], y[1], hf ? 0x7362u : 0x5140u);
-                        const uint32_t r23 = prmt(y[2], y[3], hf ? 0x7362u : 0x5140u);
-                        const uint32_t a0 = h2_lo(r01), a1 = h2_hi(r01), a2 = h2_lo(r23), a3 = h2_hi(r23);
-#pragma unroll
-                        for (int pt = 0; pt < PARTS; ++pt)
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-                                mma_f16(o[(v * 4 + w) * 2 + hf][nt], a0, a1, a2, a3, pb[pt][nt][0], pb[pt][nt][1]);
-                    }
-                }
-            }
         }
-        // merge the warps in shared memory (every copy has landed: the last NS - 1 groups are empty)
-        cp_wait<0>();
+        // merge the warps in shared memory: every copy has been waited for (after a failure, once more)
+        if (failed)
+            for (; stage != filled; stage = stage + 1 == NS ? 0 : stage + 1) {
+                mbar_wait_bounded(bar0 + 8 * stage, parity, kWaitNs);
+                parity ^= stage + 1 == NS;
+            }
         __syncthreads();
         float *osm = reinterpret_cast<float *>(smem);                              // [warps][8 NT][DP + 4]
         float2 *msm = reinterpret_cast<float2 *>(osm + kWarps * 8 * NT * (DP + 4));    // [warps][8 NT] reference, sum
@@ -544,7 +620,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const Kv8At
                 y.w = fmaf(v.w, f, y.w);
             }
             if (whole) {
-                const int tok = static_cast<int>((q0 + q) / pl.rep);
+                const int tok = static_cast<int>(div64(q0 + q, pl.rep));
                 const int hq = h * pl.rep + static_cast<int>(q0 + q - static_cast<int64_t>(tok) * pl.rep);
                 float so;
                 const float f = out_factor<MASK>(M, L, p.sinks, hq, so) * so;
@@ -555,33 +631,33 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const Kv8At
                 if (d == 0) slot_ml<DP>(p.ws, 8 * NT, G, slot)[q] = make_float2(M, L);
             }
         }
+        fence_proxy_async_smem();
         __syncthreads();                                       // before the stages are filled again
         first_seg = false;
         u += ub - ua;
     }
+    if (failed && lane == 0) atomicOr(p.r.err, 64);
 }
 
 // ---------------------------------------------------------------- the shared segments
 // One CTA per query: where several CTAs of the split kernel hold a part of its rows, adds their partials
-// in order (each warp every fourth part, four values a lane).
-constexpr int kJoinWarps = 4;
+// in order (each warp every kJoinWarps-th part, four values a lane, so up to 4 kJoinWarps parts are in flight at
+// once). The list is read before the split kernel is done (that one starts after everything before it).
+constexpr int kJoinWarps = 8;
 
-template <int DP, int NT, bool BF16, bool MASK>
+template <int DP, int NT, bool BF16, bool MASK, int R>
 __global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_kernel(const Kv8AttnParams p, int G) {
     constexpr float U = MASK ? kLog2e : 1.f;
-    constexpr int TILE = 8 * NT;
-    __shared__ float red[kJoinWarps][2];
+    constexpr int TILE = 8 * NT, V = DP == 256 ? 2 : 1;
+    __shared__ float red[kJoinWarps];
     __shared__ float4 acc[kJoinWarps][DP / 4];
-    pdl_launch_dependents();
-    pdl_wait_prerequisites();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.c.D;
-    const Plan pl(p, TILE);
-    const int q = blockIdx.x % TILE, h = blockIdx.x / TILE % p.c.Hkv, e = blockIdx.x / TILE / p.c.Hkv;
+    const Plan pl(p, TILE, kWarps * 16 * R);
+    const int q = blockIdx.x % TILE, eh = blockIdx.x / TILE, e = eh / p.c.Hkv, h = eh - e * p.c.Hkv;
     int pos, cnt;
-    const int len = pl.rows(p, e, pos, cnt), b = e / pl.tiles;
+    const int len = pl.rows(p, e, pos, cnt), b = pl.tiles == 1 ? e : e / pl.tiles;
     const int64_t qr = static_cast<int64_t>(e - b * pl.tiles) * TILE + q;
-    if (len == 0 || qr >= static_cast<int64_t>(cnt) * pl.rep) return;
-    const int n = (len - 1) / kUnit + 1;
+    const int n = (len + kWarps * 16 * R - 1) / (kWarps * 16 * R);
     int64_t before = 0, all = 0;
     for (int i = lane; i < pl.entries; i += 32) {
         const int v = pl.units(p, i);
@@ -589,18 +665,22 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_kernel(const Kv
         if (i < e) before += v;
     }
     const int64_t N = warp_sum64(all) * p.c.Hkv, u = warp_sum64(before) * p.c.Hkv + static_cast<int64_t>(h) * n;
-    const int W = static_cast<int>(min(N, static_cast<int64_t>(G)));
-    const int i0 = cta_of(N, u, W), i1 = cta_of(N, u + n - 1, W);
+    const int64_t per = units_per_cta(N, G);
+    const bool here = len > 0 && qr < static_cast<int64_t>(cnt) * pl.rep;
+    const int i0 = here ? static_cast<int>(div64(u, per)) : 0, i1 = here ? static_cast<int>(div64(u + n - 1, per)) : 0;
+    const int s0 = 2 * i0 + (i0 * per < u ? 1 : 0);            // a CTA's first segment is in its slot 0, its last in slot 1
+    const auto slot = [&](int i) { return i == i0 ? s0 : 2 * i; };
+    const int tok = static_cast<int>(div64(qr, pl.rep)), hq = h * pl.rep + static_cast<int>(qr - static_cast<int64_t>(tok) * pl.rep);
+    pdl_wait_prerequisites();
+    pdl_launch_dependents();
     if (i0 == i1) return;                                      // one CTA had it all and wrote the output
-    // a CTA's first segment is in its slot 0, a later one that it shares (its last) in slot 1
-    const auto slot = [&](int i) { return 2 * i + (i == i0 && cta_first(N, i, W) < u ? 1 : 0); };
     float M = -INFINITY;
     for (int i = i0 + lane; i <= i1; i += 32) M = fmaxf(M, slot_ml<DP>(p.ws, TILE, G, slot(i))[q].x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     const float ref = M == -INFINITY ? 0.f : M;
     float L = 0.f;
-    float4 y[DP == 256 ? 2 : 1];
+    float4 y[V];
 #pragma unroll
     for (auto &v : y) v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -610,7 +690,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_kernel(const Kv
         const float f = ex2((ml.x - ref) * U);
         L = fmaf(ml.y, f, L);
 #pragma unroll
-        for (int k = 0; k < (DP == 256 ? 2 : 1); ++k) {
+        for (int k = 0; k < V; ++k) {
             const int d = 128 * k + 4 * lane;
             if (d < D) {
                 const float4 v = *reinterpret_cast<const float4 *>(slot_o<DP>(p.ws, TILE, s) + q * DP + d);
@@ -621,28 +701,28 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_kernel(const Kv
             }
         }
     }
-    if (lane == 0) red[warp][0] = L;
+    if (lane == 0) red[warp] = L;
 #pragma unroll
-    for (int k = 0; k < (DP == 256 ? 2 : 1); ++k)
+    for (int k = 0; k < V; ++k)
         if (32 * k + lane < DP / 4) acc[warp][32 * k + lane] = y[k];
     __syncthreads();
-    L = 0.f;
-    for (int w = 0; w < kJoinWarps; ++w) L += red[w][0];
-    const int tok = static_cast<int>(qr / pl.rep), hq = h * pl.rep + static_cast<int>(qr - static_cast<int64_t>(tok) * pl.rep);
-    float so;
-    const float f = out_factor<MASK>(M, L, p.sinks, hq, so) * so;
     const int d = 4 * threadIdx.x;
     if (d < D) {
-        float4 t = acc[0][threadIdx.x];
+        L = red[0];
+        float4 s = acc[0][threadIdx.x];
+#pragma unroll
         for (int w = 1; w < kJoinWarps; ++w) {
             const float4 v = acc[w][threadIdx.x];
-            t.x += v.x;
-            t.y += v.y;
-            t.z += v.z;
-            t.w += v.w;
+            L += red[w];
+            s.x += v.x;
+            s.y += v.y;
+            s.z += v.z;
+            s.w += v.w;
         }
+        float so;
+        const float f = out_factor<MASK>(M, L, p.sinks, hq, so) * so;
         store4<BF16>(p.out, (static_cast<int64_t>(b) * p.r.T + tok) * p.ldo + static_cast<int64_t>(hq) * D + d,
-                     make_float4(t.x * f, t.y * f, t.z * f, t.w * f));
+                     make_float4(s.x * f, s.y * f, s.z * f, s.w * f));
     }
 }
 
@@ -658,22 +738,40 @@ int device_sms() {
 }
 
 // Query tiles: 8 NT queries; larger ones share the decoded codes and are limited by registers (the queries'
-// fragments take DP / 8 * NT * parts, the outputs DP / 4 * NT of them).
-int pick_nt(int DP, int64_t queries, bool bf16) {
-    const int most = DP == 64 ? 4 : DP == 128 ? (bf16 ? 4 : 2) : (bf16 ? 2 : 1);
+// digits take 3 DP / 16 * NT, the outputs DP / 4 * NT of them).
+int pick_nt(int DP, int64_t queries) {
+    const int most = DP == 64 ? 4 : DP == 128 ? 2 : 1;
     const int want = queries <= 8 ? 1 : queries <= 16 ? 2 : 4;
     return want < most ? want : most;
 }
 int padded_dim(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
+// a map of [batch][heads][rows][dim] codes whose boxes are `rows` rows of at most 128 codes, chunks exchanged
+// within a row; columns and rows past the ends read 0
+bool code_map(CUtensorMap &map, const Kv8Cache &c, int8_t *codes, int DP, int rows) {
+    const auto fn = tensor_map_encode_fn();
+    if (!fn) return false;
+    const cuuint32_t box[4] = {static_cast<cuuint32_t>(DP < 128 ? DP : 128), static_cast<cuuint32_t>(rows), 1, 1};
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.D), static_cast<cuuint64_t>(c.S), static_cast<cuuint64_t>(c.Hkv),
+                                static_cast<cuuint64_t>(c.B)};
+    // a lone head's or sequence's stride is not used: any valid one
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(c.rs), static_cast<cuuint64_t>(c.Hkv > 1 ? c.hs : c.rs),
+                                   static_cast<cuuint64_t>(c.B > 1 ? c.bs : c.rs)};
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    return fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, codes, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              DP == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int DP, int NT, bool BF16, bool MASK>
 struct Split {
-    static constexpr int NS = DP == 256 ? 3 : 4;
-    static constexpr int ring = kWarps * NS * kStageBytes<DP>, merge = kMergeBytes<DP, NT>;
-    static constexpr int smem = ring > merge ? ring : merge;
+    // rows a warp takes in a step, stages: 12 warps per SM (the registers' limit for small tiles) x 2 x 8 KB
+    static constexpr int R = DP == 256 || NT == 4 ? 1 : 2, NS = R == 1 ? 3 : 2;
+    static constexpr int ring = kWarps * NS * kStageBytes<DP, R>, merge = kMergeBytes<DP, NT>;
+    static constexpr int smem = 1024 + (ring > merge ? ring : merge);
     static int ctas() {                                        // one resident wave
         static const int n = [] {
-            auto k = kv8_attn_split_kernel<DP, NT, BF16, MASK, NS>;
+            auto k = kv8_attn_split_kernel<DP, NT, BF16, MASK, R, NS>;
             int per = 0;
             if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
                 cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, k, kWarps * 32, smem) != cudaSuccess || per < 1)
@@ -686,21 +784,24 @@ struct Split {
         const int G = ctas(), rep = p.Hq / p.c.Hkv;
         const int64_t tiles = (static_cast<int64_t>(p.r.T) * rep + 8 * NT - 1) / (8 * NT);
         const int64_t joins = tiles * p.c.B * p.c.Hkv * 8 * NT;
-        if (tiles * p.c.B > 0x7fffffff || joins > 0x7fffffff) return cudaErrorInvalidConfiguration;
-        const cudaError_t e = launch_pdl(kv8_attn_split_kernel<DP, NT, BF16, MASK, NS>, dim3(G), dim3(kWarps * 32), smem, s, p);
+        if (joins > 0x7fffffff) return cudaErrorInvalidConfiguration;
+        CUtensorMap mk, mv;
+        if (!code_map(mk, p.c, p.c.k, DP, 16 * R) || !code_map(mv, p.c, p.c.v, DP, 16 * R)) return cudaErrorInvalidValue;
+        const cudaError_t e = launch_pdl(kv8_attn_split_kernel<DP, NT, BF16, MASK, R, NS>, dim3(G), dim3(kWarps * 32), smem, s,
+                                         mk, mv, p);
         if (e != cudaSuccess) return e;
-        return launch_pdl(kv8_attn_join_kernel<DP, NT, BF16, MASK>, dim3(static_cast<unsigned>(joins)), dim3(kJoinWarps * 32),
-                          0, s, p, G);
+        return launch_pdl(kv8_attn_join_kernel<DP, NT, BF16, MASK, R>, dim3(static_cast<unsigned>(joins)),
+                          dim3(kJoinWarps * 32), 0, s, p, G);
     }
 };
 
 // f(Split<...>) for the call's sizes and types
 template <int DP, bool BF16, bool MASK, typename F>
 auto with_nt(int nt, F f) {
-    if constexpr (DP == 64 || (DP == 128 && BF16)) {
+    if constexpr (DP == 64) {
         if (nt == 4) return f(Split<DP, 4, BF16, MASK>{});
     }
-    if constexpr (DP != 256 || BF16) {
+    if constexpr (DP != 256) {
         if (nt == 2) return f(Split<DP, 2, BF16, MASK>{});
     }
     return f(Split<DP, 1, BF16, MASK>{});
@@ -712,7 +813,7 @@ auto with_types(int nt, bool bf16, bool mask, F f) {
 }
 template <typename F>
 auto with_split(int D, int64_t queries, bool bf16, bool mask, F f) {
-    const int DP = padded_dim(D), nt = pick_nt(DP, queries, bf16);
+    const int DP = padded_dim(D), nt = pick_nt(DP, queries);
     return DP == 64    ? with_types<64>(nt, bf16, mask, f)
            : DP == 128 ? with_types<128>(nt, bf16, mask, f)
                        : with_types<256>(nt, bf16, mask, f);
@@ -722,7 +823,7 @@ auto with_split(int D, int64_t queries, bool bf16, bool mask, F f) {
 
 int64_t kv8_attn_ws_bytes(int Hq, int Hkv, int D, int T, bool bf16) {
     const int64_t queries = static_cast<int64_t>(T) * (Hq / Hkv);
-    const int DP = padded_dim(D), tile = 8 * pick_nt(DP, queries, bf16);
+    const int DP = padded_dim(D), tile = 8 * pick_nt(DP, queries);
     int64_t G = 0;
     for (const bool mask : {false, true}) {
         const int64_t g = with_split(D, queries, bf16, mask, [](auto k) { return k.ctas(); });

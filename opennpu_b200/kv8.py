@@ -54,7 +54,7 @@ class KVCache8:
                   t.stride() == k_scale.stride() and (t.stride(2) == 1 or nb == 1),
                   "scales: fp32 [B, heads, ceil(rows / block)] beside k, dense along the blocks")
         self.k, self.v, self.k_scale, self.v_scale, self.block = k, v, k_scale, v_scale, block
-        self.batch, self.heads, self.rows, self.dim, self.device = B, H, S, D, k.device
+        self.batch, self.heads, self.rows, self.dim, self.device, self._dev = B, H, S, D, k.device, k.get_device()
         step = lambda t, i: t.stride(i) if t.shape[i] > 1 else 0      # a lone entry's stride says nothing
         self._desc = L.Kv8Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), B, H, S, D,
                                 step(k, 0), step(k, 1), step(k, 2) or D, step(k_scale, 0), step(k_scale, 1), block)
@@ -64,28 +64,40 @@ class KVCache8:
         self._ws = {}                     # (Hq, T, bf16) -> workspace bytes of attn
 
     # ---------------------------------------------------------------- arguments
+    # One condition a tensor: these run before every launch of a decode step.
     def _places(self, pos, cnt):
-        for t, name in ((pos, "pos"), (cnt, "cnt")):
-            if t is not None or name == "pos":
-                _need(t.dtype == torch.int32 and t.shape == (self.batch,) and t.device == self.device and
-                      (t.stride(0) == 1 or self.batch == 1), name + ": int32 [B] on the cache's device, dense")
-        return pos.data_ptr(), None if cnt is None else cnt.data_ptr()
+        shape, dev = (self.batch,), self._dev
+        for t in (pos, cnt):
+            if t is None and t is not pos:
+                return pos.data_ptr(), None
+            if t is None or t.dtype is not torch.int32 or t.shape != shape or t.get_device() != dev or \
+                    not t.is_contiguous():
+                raise L.OnpuError("pos, cnt: int32 [B] on the cache's device, dense")
+        return pos.data_ptr(), cnt.data_ptr()
 
-    def _tokens(self, t, heads, name, like=None):
+    def _tokens(self, t, heads, name):
         """The token stride of a [B, T, heads, dim] view."""
-        _need(t.dim() == 4 and t.shape[0] == self.batch and (heads is None or t.shape[2] == heads) and
-              t.shape[3] == self.dim and t.dtype in (torch.bfloat16, torch.float32) and t.device == self.device,
-              f"{name}: bf16 or fp32 [B, T, heads, dim] on the cache's device")
-        B, T, H, D = t.shape
-        sb, st, sh, sd = t.stride()
-        _need(sd == 1 and (sh == D or H == 1) and (B == 1 or T == 0 or sb == (st if T > 1 else sb) * T),
-              f"{name}: heads dense in a token's row, one stride from token to token")
-        if like is not None:
-            _need(t.shape[:2] == like.shape[:2] and t.dtype == like.dtype, f"{name}: the tokens and type of the others")
+        try:
+            B, T, H, D = t.shape
+            sb, st, sh, sd = t.stride()
+        except ValueError:
+            raise L.OnpuError(f"{name}: [B, T, heads, dim]") from None
+        if B != self.batch or D != self.dim or H != heads or t.get_device() != self._dev or \
+                (t.dtype is not torch.bfloat16 and t.dtype is not torch.float32):
+            raise L.OnpuError(f"{name}: bf16 or fp32 [B, T, heads, dim] on the cache's device")
+        if sd != 1 or (sh != D and H > 1) or (B > 1 and T > 1 and sb != st * T):
+            raise L.OnpuError(f"{name}: heads dense in a token's row, one stride from token to token")
         return st if T > 1 else sb
 
+    def _pair(self, k, v, names):
+        ldk, ldv = self._tokens(k, self.heads, names[0]), self._tokens(v, self.heads, names[1])
+        if k.shape != v.shape or k.dtype is not v.dtype:
+            raise L.OnpuError(f"{names[0]}, {names[1]}: the same tokens and type")
+        return ldk, ldv
+
     def _stream(self, stream):
-        return (torch.cuda.current_stream(self.device) if stream is None else stream).cuda_stream
+        # torch.cuda.current_stream(device).cuda_stream, at a twentieth of its host time (2 us)
+        return torch._C._cuda_getCurrentRawStream(self._dev) if stream is None else stream.cuda_stream
 
     # ---------------------------------------------------------------- calls
     def append(self, k, v, pos, cnt=None, stream=None):
@@ -93,9 +105,9 @@ class KVCache8:
         scale grows has its older rows re-rounded; a block's first row starts it anew, so rows that were
         appended and then dropped (rejected drafts) are simply written over."""
         p, n = self._places(pos, cnt)
-        ldk, ldv = self._tokens(k, self.heads, "k"), self._tokens(v, self.heads, "v", k)
+        ldk, ldv = self._pair(k, v, ("k", "v"))
         rc = self._lib.onpu_kv8_append_dev(self._ref, k.data_ptr(), ldk, v.data_ptr(), ldv, k.shape[1],
-                                           k.dtype == torch.bfloat16, p, n, self._stream(stream))
+                                           k.dtype is torch.bfloat16, p, n, self._stream(stream))
         if rc < 0:
             L.check(rc, "onpu_kv8_append_dev")
 
@@ -110,9 +122,9 @@ class KVCache8:
                        for _ in range(2)]
         k, v = out
         p, n = self._places(pos, cnt)
-        ldk, ldv = self._tokens(k, self.heads, "out[0]"), self._tokens(v, self.heads, "out[1]", k)
+        ldk, ldv = self._pair(k, v, ("out[0]", "out[1]"))
         rc = self._lib.onpu_kv8_read_dev(self._ref, k.data_ptr(), ldk, v.data_ptr(), ldv, k.shape[1],
-                                         k.dtype == torch.bfloat16, p, n, self._stream(stream))
+                                         k.dtype is torch.bfloat16, p, n, self._stream(stream))
         if rc < 0:
             L.check(rc, "onpu_kv8_read_dev")
         return k, v
@@ -124,21 +136,22 @@ class KVCache8:
         scale defaults to dim ** -0.5. Returns [B, T, Hq, dim] of q's type; a token whose mask leaves no
         row gets zeros, tokens at and past cnt are left as they were (undefined in a new tensor)."""
         p, n = self._places(pos, cnt)
-        ldq = self._tokens(q, None, "q")
-        B, T, Hq, D = q.shape
-        bf16 = q.dtype == torch.bfloat16
+        Hq = q.shape[2] if q.dim() == 4 else 0
+        ldq = self._tokens(q, Hq, "q")
+        B, T, D, dev, bf16 = self.batch, q.shape[1], self.dim, self._dev, q.dtype is torch.bfloat16
         mp, mbs, mts, sp = None, 0, 0, None
         if mask is not None:
-            _need(mask.dtype == torch.float32 and mask.dim() == 3 and mask.shape[0] in (1, B) and
-                  mask.shape[1] in (1, T) and mask.shape[2] == self.rows and mask.device == self.device and
-                  (mask.stride(2) == 1 or self.rows == 1),
-                  "mask: fp32 [B or 1, T or 1, rows] on the cache's device, dense along the rows")
+            if mask.dtype is not torch.float32 or mask.dim() != 3 or mask.shape[0] not in (1, B) or \
+                    mask.shape[1] not in (1, T) or mask.shape[2] != self.rows or mask.get_device() != dev or \
+                    (mask.stride(2) != 1 and self.rows > 1):
+                raise L.OnpuError("mask: fp32 [B or 1, T or 1, rows] on the cache's device, dense along the rows")
             mp = mask.data_ptr()
             mbs = mask.stride(0) if mask.shape[0] > 1 else 0
             mts = mask.stride(1) if mask.shape[1] > 1 else 0
         if sinks is not None:
-            _need(sinks.dtype == torch.float32 and sinks.shape == (Hq,) and sinks.device == self.device and
-                  (sinks.stride(0) == 1 or Hq == 1), "sinks: fp32 [Hq] on the cache's device, dense")
+            if sinks.dtype is not torch.float32 or sinks.shape != (Hq,) or sinks.get_device() != dev or \
+                    not sinks.is_contiguous():
+                raise L.OnpuError("sinks: fp32 [Hq] on the cache's device, dense")
             sp = sinks.data_ptr()
         size = self._ws.get((Hq, T, bf16))
         if size is None:
@@ -151,7 +164,9 @@ class KVCache8:
             with torch.cuda.stream(stream):        # memory that this stream may use again
                 ws = torch.empty(size, dtype=torch.uint8, device=self.device)
                 out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=self.device) if out is None else out
-        ldo = self._tokens(out, Hq, "out", q)
+        ldo = self._tokens(out, Hq, "out")
+        if out.shape[1] != T or out.dtype is not q.dtype:
+            raise L.OnpuError("out: q's tokens and type")
         rc = self._lib.onpu_kv8_attn_dev(self._ref, q.data_ptr(), ldq, Hq, T, bf16, p, n, mp, mbs, mts, sp,
                                          D ** -0.5 if scale is None else scale, out.data_ptr(), ldo, ws.data_ptr(),
                                          self._stream(stream))
