@@ -1,7 +1,10 @@
 // Device helpers the 8-bit KV cache's kernels share.
 #pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdint>
 
 #include "kernels.h"
@@ -16,6 +19,198 @@ __device__ __forceinline__ bool kv8_rows(const Kv8Rows &r, int b, int S, int &po
     if (cnt >= 0 && cnt <= r.T && pos >= 0 && pos <= S - cnt) return true;
     atomicOr(r.err, 32);
     return false;
+}
+
+// ---------------------------------------------------------------- attention
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint64_t kWaitNs = 2000000000ull;   // bound of every wait for a copy
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+    uint32_t d;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
+    return d;
+}
+// two biased codes u = c + 128 in bytes (lo: 0 and 1, hi: 2 and 3 of x) -> fp16 pair c: 0x64uu is 1024 + u
+__device__ __forceinline__ uint32_t h2_lo(uint32_t x) {
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(prmt(x, 0x64646464u, 0x4140u)), "r"(0x64806480u));
+    return d;
+}
+__device__ __forceinline__ uint32_t h2_hi(uint32_t x) {
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(prmt(x, 0x64646464u, 0x4342u)), "r"(0x64806480u));
+    return d;
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 unpack_h2(uint32_t x) { return __half22float2(*reinterpret_cast<__half2 *>(&x)); }
+// 2^(top - exponent of x), its exponent kept within +-100: x times it is in [2^top, 2^(top + 1)); 1 for 0, inf and NaN
+__device__ __forceinline__ float pow2_to(float x, int top) {
+    const int e = static_cast<int>(__float_as_uint(x) >> 23 & 0xff);
+    if (e == 255 || !(fabsf(x) > 0.f)) return 1.f;
+    return __uint_as_float(static_cast<uint32_t>(127 + min(100, max(-100, top + 127 - e))) << 23);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {     // NaN where either is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// ---------------------------------------------------------------- the list of units
+// An entry is a (sequence, query tile); its rows are counted in units of `unit` rows, once per kv head.
+struct Plan {
+    int rep, tile, tiles, entries, unit;    // query heads per kv head, queries a tile, tiles a sequence, B * tiles
+    __device__ __forceinline__ Plan(const Kv8AttnParams &p, int tile_, int unit_) {
+        rep = p.Hq / p.c.Hkv;
+        tile = tile_;
+        unit = unit_;
+        tiles = static_cast<int>((static_cast<int64_t>(p.r.T) * rep + tile - 1) / tile);
+        entries = p.c.B * tiles;
+    }
+    // rows that entry e's tile sees (0: nothing of it is valid)
+    __device__ __forceinline__ int rows(const Kv8AttnParams &p, int e, int &pos, int &cnt) const {
+        const int b = tiles == 1 ? e : e / tiles;
+        if (!kv8_rows(p.r, b, p.c.S, pos, cnt)) return 0;
+        if (tiles == 1) return cnt > 0 ? pos + cnt : 0;
+        const int64_t r0 = static_cast<int64_t>(e - b * tiles) * tile;
+        const int first = static_cast<int>(r0 / rep), last = static_cast<int>((r0 + tile - 1) / rep);
+        if (first >= cnt) return 0;
+        return pos + min(last, cnt - 1) + 1;
+    }
+    __device__ __forceinline__ int units(const Kv8AttnParams &p, int e) const {
+        int pos, cnt;
+        const unsigned n = rows(p, e, pos, cnt);
+        return static_cast<int>((n + unit - 1) / unit);
+    }
+};
+__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// a / b, in 32 bits where they fit (they all but always do; a 64-bit division costs a few hundred instructions)
+__device__ __forceinline__ int64_t div64(int64_t a, int64_t b) {
+    if (((a | b) >> 31) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+// units a CTA takes: N units over G CTAs, at least kMinUnits each (a part shorter than that costs more to
+// join than it saves); CTA i has units [i * per, (i + 1) * per) of the list
+constexpr int kMinUnits = 1;
+__device__ __forceinline__ int64_t units_per_cta(int64_t N, int G) {
+    return max(static_cast<int64_t>(kMinUnits), div64(N + G - 1, G));
+}
+
+// ws: per CTA two slots of [tile][DP] outputs, then per slot [tile] (reference, sum) pairs
+template <int DP>
+__device__ __forceinline__ float *slot_o(void *ws, int tile, int slot) {
+    return static_cast<float *>(ws) + static_cast<int64_t>(slot) * tile * DP;
+}
+template <int DP>
+__device__ __forceinline__ float2 *slot_ml(void *ws, int tile, int G, int slot) {
+    return reinterpret_cast<float2 *>(static_cast<float *>(ws) + static_cast<int64_t>(2) * G * tile * DP) +
+           static_cast<int64_t>(slot) * tile;
+}
+// Where CTA i of the list stands: the entry that holds unit u (every lane of the warp gets it), its units
+// and its first one
+__device__ __forceinline__ void find_entry(const Kv8AttnParams &p, const Plan &pl, int lane, int64_t u, int &e, int &n,
+                                           int64_t &e0) {
+    e0 = 0;
+    for (int base = 0;; base += 32) {
+        const int mine = base + lane < pl.entries ? pl.units(p, base + lane) : 0;
+        int64_t incl = static_cast<int64_t>(mine) * p.c.Hkv;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += up;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, e0 + incl > u);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            n = __shfl_sync(0xffffffffu, mine, src);
+            e0 += __shfl_sync(0xffffffffu, incl, src) - static_cast<int64_t>(n) * p.c.Hkv;
+            e = base + src;
+            return;
+        }
+        e0 += __shfl_sync(0xffffffffu, incl, 31);
+    }
+}
+// units of all entries and heads
+__device__ __forceinline__ int64_t total_units(const Kv8AttnParams &p, const Plan &pl, int lane) {
+    int64_t N = 0;
+    for (int e = lane; e < pl.entries; e += 32) N += pl.units(p, e);
+    return warp_sum64(N) * p.c.Hkv;
+}
+// A CTA's way through the list: segments, each a run of one entry's units for one kv head
+struct Walk {
+    int64_t u, u1, e0;                // the next unit, the end of this CTA's, the entry's first
+    int e, n;                         // the entry and its units (per head)
+    bool first;                       // no segment taken yet
+    // the segment at u
+    int b, h, ua, ub, pos, cnt, len, nq;
+    int64_t q0;                       // the tile's first query
+    __device__ __forceinline__ bool start(const Kv8AttnParams &p, const Plan &pl, int lane, int cta, int G) {
+        const int64_t N = total_units(p, pl, lane), per = units_per_cta(N, G);
+        u = per * cta;
+        u1 = min(N, u + per);
+        if (u >= u1) return false;
+        find_entry(p, pl, lane, u, e, n, e0);
+        first = true;
+        return true;
+    }
+    __device__ __forceinline__ bool segment(const Kv8AttnParams &p, const Plan &pl) {
+        if (u >= u1) return false;
+        while (n == 0 || u >= e0 + static_cast<int64_t>(n) * p.c.Hkv) {     // the next entry with rows
+            e0 += static_cast<int64_t>(n) * p.c.Hkv;
+            n = pl.units(p, ++e);
+        }
+        h = static_cast<int>(div64(u - e0, n));
+        ua = static_cast<int>(u - e0 - static_cast<int64_t>(h) * n);
+        ub = static_cast<int>(min(static_cast<int64_t>(n), ua + (u1 - u)));
+        len = pl.rows(p, e, pos, cnt);
+        b = pl.tiles == 1 ? e : e / pl.tiles;
+        q0 = static_cast<int64_t>(e - b * pl.tiles) * pl.tile;
+        nq = static_cast<int>(min(static_cast<int64_t>(pl.tile), static_cast<int64_t>(cnt) * pl.rep - q0));
+        return true;
+    }
+    __device__ __forceinline__ bool whole() const { return ua == 0 && ub == n; }
+    __device__ __forceinline__ int slot(int cta) const { return 2 * cta + (first ? 0 : 1); }
+    __device__ __forceinline__ void next() {
+        first = false;
+        u += ub - ua;
+    }
+};
+
+
+template <bool BF16>
+__device__ __forceinline__ void store4(void *out, int64_t o, float4 y) {
+    if constexpr (BF16) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
+        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(out) + o) =
+            make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    } else {
+        *reinterpret_cast<float4 *>(static_cast<float *>(out) + o) = y;
+    }
+}
+// sums -> outputs: divide by the sum and the sink's share, zeros where nothing is left
+template <bool MASK>
+__device__ __forceinline__ float out_factor(float M, float Lsum, const float *sinks, int hq, float &scale_o) {
+    // returns 1 / total and, in scale_o, the factor that takes sums relative to M onto the common reference
+    float total = Lsum;
+    scale_o = 1.f;
+    if (sinks) {
+        const float sk = MASK ? sinks[hq] : sinks[hq] * kLog2e, U = MASK ? kLog2e : 1.f;
+        const float top = fmaxf(M, sk), ref = top == -INFINITY ? 0.f : top;
+        scale_o = ex2((M - ref) * U);
+        total = Lsum * scale_o + ex2((sk - ref) * U);
+    }
+    return total == 0.f ? 0.f : 1.f / total;
 }
 
 }  // namespace onpu_b200

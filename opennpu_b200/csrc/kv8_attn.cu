@@ -30,6 +30,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "kernels.h"
 #include "kv8.cuh"
@@ -40,30 +41,7 @@ namespace onpu_b200 {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr uint64_t kWaitNs = 2000000000ull;   // bound of every wait for a copy
-constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-    uint32_t d;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
-    return d;
-}
-// two biased codes u = c + 128 in bytes (lo: 0 and 1, hi: 2 and 3 of x) -> fp16 pair c: 0x64uu is 1024 + u
-__device__ __forceinline__ uint32_t h2_lo(uint32_t x) {
-    uint32_t d;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(prmt(x, 0x64646464u, 0x4140u)), "r"(0x64806480u));
-    return d;
-}
-__device__ __forceinline__ uint32_t h2_hi(uint32_t x) {
-    uint32_t d;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(prmt(x, 0x64646464u, 0x4342u)), "r"(0x64806480u));
-    return d;
-}
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -75,103 +53,6 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
     return d;
 }
-__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ float2 unpack_h2(uint32_t x) { return __half22float2(*reinterpret_cast<__half2 *>(&x)); }
-// 2^(top - exponent of x), its exponent kept within +-100: x times it is in [2^top, 2^(top + 1)); 1 for 0, inf and NaN
-__device__ __forceinline__ float pow2_to(float x, int top) {
-    const int e = static_cast<int>(__float_as_uint(x) >> 23 & 0xff);
-    if (e == 255 || !(fabsf(x) > 0.f)) return 1.f;
-    return __uint_as_float(static_cast<uint32_t>(127 + min(100, max(-100, top + 127 - e))) << 23);
-}
-__device__ __forceinline__ float max_nan(float a, float b) {     // NaN where either is
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-
-// ---------------------------------------------------------------- the list of units
-// An entry is a (sequence, query tile); its rows are counted in units of kWarps * 16 R, once per kv head.
-struct Plan {
-    int rep, tile, tiles, entries, unit;    // query heads per kv head, queries a tile, tiles a sequence, B * tiles
-    __device__ __forceinline__ Plan(const Kv8AttnParams &p, int tile_, int unit_) {
-        rep = p.Hq / p.c.Hkv;
-        tile = tile_;
-        unit = unit_;
-        tiles = static_cast<int>((static_cast<int64_t>(p.r.T) * rep + tile - 1) / tile);
-        entries = p.c.B * tiles;
-    }
-    // rows that entry e's tile sees (0: nothing of it is valid)
-    __device__ __forceinline__ int rows(const Kv8AttnParams &p, int e, int &pos, int &cnt) const {
-        const int b = tiles == 1 ? e : e / tiles;
-        if (!kv8_rows(p.r, b, p.c.S, pos, cnt)) return 0;
-        if (tiles == 1) return cnt > 0 ? pos + cnt : 0;
-        const int64_t r0 = static_cast<int64_t>(e - b * tiles) * tile;
-        const int first = static_cast<int>(r0 / rep), last = static_cast<int>((r0 + tile - 1) / rep);
-        if (first >= cnt) return 0;
-        return pos + min(last, cnt - 1) + 1;
-    }
-    __device__ __forceinline__ int units(const Kv8AttnParams &p, int e) const {
-        int pos, cnt;
-        const unsigned n = rows(p, e, pos, cnt);
-        return static_cast<int>((n + unit - 1) / unit);
-    }
-};
-__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-// a / b, in 32 bits where they fit (they all but always do; a 64-bit division costs a few hundred instructions)
-__device__ __forceinline__ int64_t div64(int64_t a, int64_t b) {
-    if (((a | b) >> 31) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-    return a / b;
-}
-// units a CTA takes: N units over G CTAs, at least kMinUnits each (a part shorter than that costs more to
-// join than it saves); CTA i has units [i * per, (i + 1) * per) of the list
-constexpr int kMinUnits = 1;
-__device__ __forceinline__ int64_t units_per_cta(int64_t N, int G) {
-    return max(static_cast<int64_t>(kMinUnits), div64(N + G - 1, G));
-}
-
-// ws: per CTA two slots of [tile][DP] outputs, then per slot [tile] (reference, sum) pairs
-template <int DP>
-__device__ __forceinline__ float *slot_o(void *ws, int tile, int slot) {
-    return static_cast<float *>(ws) + static_cast<int64_t>(slot) * tile * DP;
-}
-template <int DP>
-__device__ __forceinline__ float2 *slot_ml(void *ws, int tile, int G, int slot) {
-    return reinterpret_cast<float2 *>(static_cast<float *>(ws) + static_cast<int64_t>(2) * G * tile * DP) +
-           static_cast<int64_t>(slot) * tile;
-}
-
-template <bool BF16>
-__device__ __forceinline__ void store4(void *out, int64_t o, float4 y) {
-    if constexpr (BF16) {
-        const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
-        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(out) + o) =
-            make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
-    } else {
-        *reinterpret_cast<float4 *>(static_cast<float *>(out) + o) = y;
-    }
-}
-// sums -> outputs: divide by the sum and the sink's share, zeros where nothing is left
-template <bool MASK>
-__device__ __forceinline__ float out_factor(float M, float Lsum, const float *sinks, int hq, float &scale_o) {
-    // returns 1 / total and, in scale_o, the factor that takes sums relative to M onto the common reference
-    float total = Lsum;
-    scale_o = 1.f;
-    if (sinks) {
-        const float sk = MASK ? sinks[hq] : sinks[hq] * kLog2e, U = MASK ? kLog2e : 1.f;
-        const float top = fmaxf(M, sk), ref = top == -INFINITY ? 0.f : top;
-        scale_o = ex2((M - ref) * U);
-        total = Lsum * scale_o + ex2((sk - ref) * U);
-    }
-    return total == 0.f ? 0.f : 1.f / total;
-}
-
 // ---------------------------------------------------------------- the split kernel
 // A stage: 16 R rows of K, then of V, as TMA wrote them: rows of 64 or 128 bytes (256: two such halves one
 // after the other), their 16-byte chunks exchanged by the map's swizzle.
@@ -231,56 +112,21 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __gri
     pdl_launch_dependents();              // after the wait: the join may read pos and cnt as it starts
 
     const Plan pl(p, 8 * NT, kWarps * ROWS);
-    // units of all entries and heads
-    int64_t N = 0;
-    for (int e = lane; e < pl.entries; e += 32) N += pl.units(p, e);
-    N = warp_sum64(N) * c.Hkv;
-    const int64_t per = units_per_cta(N, G);
-    int64_t u = per * blockIdx.x;
-    const int64_t u1 = min(N, u + per);
-    if (u >= u1) return;
-    // the entry that holds unit u, and its first unit
-    int e = 0, n = 0;
-    int64_t e0 = 0;
-    for (int base = 0;; base += 32) {
-        const int mine = base + lane < pl.entries ? pl.units(p, base + lane) : 0;
-        int64_t incl = static_cast<int64_t>(mine) * c.Hkv;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += up;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, e0 + incl > u);
-        if (hit) {
-            const int src = __ffs(hit) - 1;
-            n = __shfl_sync(0xffffffffu, mine, src);
-            e0 += __shfl_sync(0xffffffffu, incl, src) - static_cast<int64_t>(n) * c.Hkv;
-            e = base + src;
-            break;
-        }
-        e0 += __shfl_sync(0xffffffffu, incl, 31);
-    }
+    Walk wk;
+    if (!wk.start(p, pl, lane, blockIdx.x, G)) return;
 
-    bool first_seg = true, failed = false;
+    bool failed = false;
     int stage = 0, filled = 0;                     // the next stage to read and its parity, the next to fill
     uint32_t parity = 0;
     // this lane's rows of a 16-row block: for V (4 of them) and, of those that lanes 4 (g / 2) .. hold, for K
     // (two). Rows 2p and (2p ^ 4) + 1 [+ 8]: in the swizzled tile the eight lanes of a phase never meet in a bank.
     const int vr0 = 2 * t, vr1 = ((2 * t) ^ 4) + 1;
     const int kp = g >> 1, ra = g & 1 ? ((2 * kp) ^ 4) + 1 : 2 * kp, rb = ra + 8;
-    while (u < u1) {
-        while (n == 0 || u >= e0 + static_cast<int64_t>(n) * c.Hkv) {     // the next entry with rows
-            e0 += static_cast<int64_t>(n) * c.Hkv;
-            n = pl.units(p, ++e);
-        }
-        const int h = static_cast<int>(div64(u - e0, n)), ua = static_cast<int>(u - e0 - static_cast<int64_t>(h) * n);
-        const int ub = static_cast<int>(min(static_cast<int64_t>(n), ua + (u1 - u)));
-        int pos, cnt;
-        const int len = pl.rows(p, e, pos, cnt), b = pl.tiles == 1 ? e : e / pl.tiles;
-        const int64_t q0 = static_cast<int64_t>(e - b * pl.tiles) * pl.tile;         // the tile's first query
-        const int nq = static_cast<int>(min(static_cast<int64_t>(pl.tile), static_cast<int64_t>(cnt) * pl.rep - q0));
-        const int row0 = ua * kWarps * ROWS;
-        const int row1 = static_cast<int>(min(static_cast<int64_t>(len), static_cast<int64_t>(ub) * kWarps * ROWS));
+    for (; wk.segment(p, pl); wk.next()) {
+        const int b = wk.b, h = wk.h, pos = wk.pos, nq = wk.nq;
+        const int64_t q0 = wk.q0;
+        const int row0 = wk.ua * kWarps * ROWS;
+        const int row1 = static_cast<int>(min(static_cast<int64_t>(wk.len), static_cast<int64_t>(wk.ub) * kWarps * ROWS));
         const int nstep = (row1 - row0 + ROWS - 1) / ROWS;
         const float *ksb = c.ks + b * c.sbs + h * c.shs, *vsb = c.vs + b * c.sbs + h * c.shs;
 
@@ -597,8 +443,8 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __gri
                 }
             }
         __syncthreads();
-        const bool whole = ua == 0 && ub == n;
-        const int slot = 2 * blockIdx.x + (first_seg ? 0 : 1);
+        const bool whole = wk.whole();
+        const int slot = wk.slot(blockIdx.x);
         const int dv = D >> 2;
         for (int i = threadIdx.x; i < nq * dv; i += kWarps * 32) {
             const int q = i / dv, d = (i - q * dv) * 4;
@@ -633,8 +479,6 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __gri
         }
         fence_proxy_async_smem();
         __syncthreads();                                       // before the stages are filled again
-        first_seg = false;
-        u += ub - ua;
     }
     if (failed && lane == 0) atomicOr(p.r.err, 64);
 }
@@ -645,19 +489,19 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __gri
 // once). The list is read before the split kernel is done (that one starts after everything before it).
 constexpr int kJoinWarps = 8;
 
-template <int DP, int NT, bool BF16, bool MASK, int R>
-__global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_kernel(const Kv8AttnParams p, int G) {
+template <int DP, bool BF16, bool MASK>
+__global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_kernel(const Kv8AttnParams p, int G, int tile, int unit) {
     constexpr float U = MASK ? kLog2e : 1.f;
-    constexpr int TILE = 8 * NT, V = DP == 256 ? 2 : 1;
+    constexpr int V = DP == 256 ? 2 : 1;
     __shared__ float red[kJoinWarps];
     __shared__ float4 acc[kJoinWarps][DP / 4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.c.D;
-    const Plan pl(p, TILE, kWarps * 16 * R);
-    const int q = blockIdx.x % TILE, eh = blockIdx.x / TILE, e = eh / p.c.Hkv, h = eh - e * p.c.Hkv;
+    const Plan pl(p, tile, unit);
+    const int eh = blockIdx.x / tile, q = blockIdx.x - eh * tile, e = eh / p.c.Hkv, h = eh - e * p.c.Hkv;
     int pos, cnt;
     const int len = pl.rows(p, e, pos, cnt), b = pl.tiles == 1 ? e : e / pl.tiles;
-    const int64_t qr = static_cast<int64_t>(e - b * pl.tiles) * TILE + q;
-    const int n = (len + kWarps * 16 * R - 1) / (kWarps * 16 * R);
+    const int64_t qr = static_cast<int64_t>(e - b * pl.tiles) * tile + q;
+    const int n = static_cast<int>((static_cast<unsigned>(len) + unit - 1) / unit);
     int64_t before = 0, all = 0;
     for (int i = lane; i < pl.entries; i += 32) {
         const int v = pl.units(p, i);
@@ -675,7 +519,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_kernel(const Kv
     pdl_launch_dependents();
     if (i0 == i1) return;                                      // one CTA had it all and wrote the output
     float M = -INFINITY;
-    for (int i = i0 + lane; i <= i1; i += 32) M = fmaxf(M, slot_ml<DP>(p.ws, TILE, G, slot(i))[q].x);
+    for (int i = i0 + lane; i <= i1; i += 32) M = fmaxf(M, slot_ml<DP>(p.ws, tile, G, slot(i))[q].x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     const float ref = M == -INFINITY ? 0.f : M;
@@ -686,14 +530,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_kernel(const Kv
 #pragma unroll 4
     for (int i = i0 + warp; i <= i1; i += kJoinWarps) {
         const int s = slot(i);
-        const float2 ml = slot_ml<DP>(p.ws, TILE, G, s)[q];
+        const float2 ml = slot_ml<DP>(p.ws, tile, G, s)[q];
         const float f = ex2((ml.x - ref) * U);
         L = fmaf(ml.y, f, L);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const int d = 128 * k + 4 * lane;
             if (d < D) {
-                const float4 v = *reinterpret_cast<const float4 *>(slot_o<DP>(p.ws, TILE, s) + q * DP + d);
+                const float4 v = *reinterpret_cast<const float4 *>(slot_o<DP>(p.ws, tile, s) + q * DP + d);
                 y[k].x = fmaf(v.x, f, y[k].x);
                 y[k].y = fmaf(v.y, f, y[k].y);
                 y[k].z = fmaf(v.z, f, y[k].z);
@@ -740,10 +584,13 @@ int device_sms() {
 // Query tiles: 8 NT queries; larger ones share the decoded codes and are limited by registers (the queries'
 // digits take 3 DP / 16 * NT, the outputs DP / 4 * NT of them).
 int pick_nt(int DP, int64_t queries) {
-    const int most = DP == 64 ? 4 : DP == 128 ? 2 : 1;
+    const int most = DP == 64 ? 2 : DP == 128 ? 2 : 1;
     const int want = queries <= 8 ? 1 : queries <= 16 ? 2 : 4;
     return want < most ? want : most;
 }
+// more queries a kv head than this go to 128-query tiles (kv8_tile.cu), where heads fit them
+constexpr int kTileFrom = 16;
+bool use_tiles(int D, int64_t queries) { return D <= 128 && queries > kTileFrom; }
 int padded_dim(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 // a map of [batch][heads][rows][dim] codes whose boxes are `rows` rows of at most 128 codes, chunks exchanged
@@ -761,6 +608,16 @@ bool code_map(CUtensorMap &map, const Kv8Cache &c, int8_t *codes, int DP, int ro
     return fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, codes, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
               DP == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// after a split kernel of G CTAs over units of `unit` rows and tiles of `tile` queries
+template <int DP, bool BF16, bool MASK>
+cudaError_t join_launch(const Kv8AttnParams &p, int G, int tile, int unit, cudaStream_t s) {
+    const int64_t tiles = (static_cast<int64_t>(p.r.T) * (p.Hq / p.c.Hkv) + tile - 1) / tile;
+    const int64_t joins = tiles * p.c.B * p.c.Hkv * tile;
+    if (joins > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    return launch_pdl(kv8_attn_join_kernel<DP, BF16, MASK>, dim3(static_cast<unsigned>(joins)), dim3(kJoinWarps * 32), 0, s, p,
+                      G, tile, unit);
 }
 
 template <int DP, int NT, bool BF16, bool MASK>
@@ -783,15 +640,13 @@ struct Split {
     static cudaError_t launch(const Kv8AttnParams &p, cudaStream_t s) {
         const int G = ctas(), rep = p.Hq / p.c.Hkv;
         const int64_t tiles = (static_cast<int64_t>(p.r.T) * rep + 8 * NT - 1) / (8 * NT);
-        const int64_t joins = tiles * p.c.B * p.c.Hkv * 8 * NT;
-        if (joins > 0x7fffffff) return cudaErrorInvalidConfiguration;
+        if (tiles * p.c.B > 0x7fffffff) return cudaErrorInvalidConfiguration;
         CUtensorMap mk, mv;
         if (!code_map(mk, p.c, p.c.k, DP, 16 * R) || !code_map(mv, p.c, p.c.v, DP, 16 * R)) return cudaErrorInvalidValue;
         const cudaError_t e = launch_pdl(kv8_attn_split_kernel<DP, NT, BF16, MASK, R, NS>, dim3(G), dim3(kWarps * 32), smem, s,
                                          mk, mv, p);
         if (e != cudaSuccess) return e;
-        return launch_pdl(kv8_attn_join_kernel<DP, NT, BF16, MASK, R>, dim3(static_cast<unsigned>(joins)),
-                          dim3(kJoinWarps * 32), 0, s, p, G);
+        return join_launch<DP, BF16, MASK>(p, G, 8 * NT, kWarps * 16 * R, s);
     }
 };
 
@@ -823,18 +678,34 @@ auto with_split(int D, int64_t queries, bool bf16, bool mask, F f) {
 
 int64_t kv8_attn_ws_bytes(int Hq, int Hkv, int D, int T, bool bf16) {
     const int64_t queries = static_cast<int64_t>(T) * (Hq / Hkv);
-    const int DP = padded_dim(D), tile = 8 * pick_nt(DP, queries);
-    int64_t G = 0;
-    for (const bool mask : {false, true}) {
-        const int64_t g = with_split(D, queries, bf16, mask, [](auto k) { return k.ctas(); });
-        G = g > G ? g : G;
+    const int DP = padded_dim(D);
+    int64_t G = 0, tile = 8 * pick_nt(DP, queries);
+    if (use_tiles(D, queries)) {
+        G = kv8_tile_ctas();
+        tile = kv8_tile_queries(queries, bf16);
+    } else {
+        for (const bool mask : {false, true}) {
+            const int64_t g = with_split(D, queries, bf16, mask, [](auto k) { return static_cast<int64_t>(k.ctas()); });
+            G = g > G ? g : G;
+        }
     }
     return 2 * G * tile * (DP + 2) * 4;
 }
 
-cudaError_t kv8_attn_launch(const Kv8AttnParams &p, bool bf16, cudaStream_t stream) {
-    return with_split(p.c.D, static_cast<int64_t>(p.r.T) * (p.Hq / p.c.Hkv), bf16, p.mask != nullptr,
-                      [&](auto k) { return k.launch(p, stream); });
+cudaError_t kv8_attn_launch(const Kv8AttnParams &p, bool bf16, cudaStream_t s) {
+    const int64_t queries = static_cast<int64_t>(p.r.T) * (p.Hq / p.c.Hkv);
+    if (!use_tiles(p.c.D, queries))
+        return with_split(p.c.D, queries, bf16, p.mask != nullptr, [&](auto k) { return k.launch(p, s); });
+    const int G = kv8_tile_ctas(), tile = kv8_tile_queries(queries, bf16), unit = kv8_tile_rows();
+    if ((queries + tile - 1) / tile * p.c.B > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    const cudaError_t e = kv8_tile_launch(p, bf16, s);
+    if (e != cudaSuccess) return e;
+    const auto join = [&](auto dp) {
+        constexpr int DP = decltype(dp)::value;
+        if (bf16) return p.mask ? join_launch<DP, true, true>(p, G, tile, unit, s) : join_launch<DP, true, false>(p, G, tile, unit, s);
+        return p.mask ? join_launch<DP, false, true>(p, G, tile, unit, s) : join_launch<DP, false, false>(p, G, tile, unit, s);
+    };
+    return p.c.D <= 64 ? join(std::integral_constant<int, 64>{}) : join(std::integral_constant<int, 128>{});
 }
 
 }  // namespace onpu_b200
