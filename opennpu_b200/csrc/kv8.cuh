@@ -188,6 +188,32 @@ struct Walk {
 };
 
 
+// Which CTAs hold entry e's rows for head h, and in which of their slots: a CTA's first segment is in its slot 0, its
+// last in slot 1. i0 == i1: one has them all.
+struct Shares {
+    int b, cnt, i0, i1, s0;
+    int64_t q0;                       // the tile's first query
+    __device__ __forceinline__ Shares(const Kv8AttnParams &p, const Plan &pl, int lane, int e, int h, int G) {
+        int64_t before = 0, all = 0;
+        for (int i = lane; i < pl.entries; i += 32) {
+            const int v = pl.units(p, i);
+            all += v;
+            if (i < e) before += v;
+        }
+        int pos;
+        const unsigned len = pl.rows(p, e, pos, cnt);
+        const int n = static_cast<int>((len + pl.unit - 1) / pl.unit);
+        b = pl.tiles == 1 ? e : e / pl.tiles;
+        q0 = static_cast<int64_t>(e - b * pl.tiles) * pl.tile;
+        const int64_t N = warp_sum64(all) * p.c.Hkv, u = warp_sum64(before) * p.c.Hkv + static_cast<int64_t>(h) * n;
+        const int64_t per = units_per_cta(N, G);
+        i0 = n ? static_cast<int>(div64(u, per)) : 0;
+        i1 = n ? static_cast<int>(div64(u + n - 1, per)) : 0;
+        s0 = 2 * i0 + (i0 * per < u ? 1 : 0);
+    }
+    __device__ __forceinline__ int slot(int i) const { return i == i0 ? s0 : 2 * i; }
+};
+
 template <bool BF16>
 __device__ __forceinline__ void store4(void *out, int64_t o, float4 y) {
     if constexpr (BF16) {

@@ -498,22 +498,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_kernel(const Kv
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.c.D;
     const Plan pl(p, tile, unit);
     const int eh = blockIdx.x / tile, q = blockIdx.x - eh * tile, e = eh / p.c.Hkv, h = eh - e * p.c.Hkv;
-    int pos, cnt;
-    const int len = pl.rows(p, e, pos, cnt), b = pl.tiles == 1 ? e : e / pl.tiles;
-    const int64_t qr = static_cast<int64_t>(e - b * pl.tiles) * tile + q;
-    const int n = static_cast<int>((static_cast<unsigned>(len) + unit - 1) / unit);
-    int64_t before = 0, all = 0;
-    for (int i = lane; i < pl.entries; i += 32) {
-        const int v = pl.units(p, i);
-        all += v;
-        if (i < e) before += v;
-    }
-    const int64_t N = warp_sum64(all) * p.c.Hkv, u = warp_sum64(before) * p.c.Hkv + static_cast<int64_t>(h) * n;
-    const int64_t per = units_per_cta(N, G);
-    const bool here = len > 0 && qr < static_cast<int64_t>(cnt) * pl.rep;
-    const int i0 = here ? static_cast<int>(div64(u, per)) : 0, i1 = here ? static_cast<int>(div64(u + n - 1, per)) : 0;
-    const int s0 = 2 * i0 + (i0 * per < u ? 1 : 0);            // a CTA's first segment is in its slot 0, its last in slot 1
-    const auto slot = [&](int i) { return i == i0 ? s0 : 2 * i; };
+    const Shares sh(p, pl, lane, e, h, G);
+    const int64_t qr = sh.q0 + q;
+    const int i0 = sh.i0, i1 = qr < static_cast<int64_t>(sh.cnt) * pl.rep ? sh.i1 : i0, b = sh.b;
+    const auto slot = [&](int i) { return sh.slot(i); };
     const int tok = static_cast<int>(div64(qr, pl.rep)), hq = h * pl.rep + static_cast<int>(qr - static_cast<int64_t>(tok) * pl.rep);
     pdl_wait_prerequisites();
     pdl_launch_dependents();
@@ -570,6 +558,55 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_kernel(const Kv
     }
 }
 
+// The same after kv8_tile.cu, whose many queries share a CTA's plan: kJoinRows queries a CTA, a warp at a time on
+// each of its share (one CTA a query took 161 us of a 512-token chunk's 450).
+constexpr int kJoinRows = 32;
+
+template <int DP, bool BF16, bool MASK>
+__global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_rows_kernel(const Kv8AttnParams p, int G, int tile, int unit) {
+    constexpr float U = MASK ? kLog2e : 1.f;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.c.D, groups = tile / kJoinRows;
+    const Plan pl(p, tile, unit);
+    const int eh = blockIdx.x / groups, qg = (blockIdx.x - eh * groups) * kJoinRows, e = eh / p.c.Hkv, h = eh - e * p.c.Hkv;
+    const Shares sh(p, pl, lane, e, h, G);
+    pdl_wait_prerequisites();
+    pdl_launch_dependents();
+    if (sh.i0 == sh.i1) return;                                // one CTA had it all and wrote the outputs
+    const int last = static_cast<int>(min(static_cast<int64_t>(qg + kJoinRows), static_cast<int64_t>(sh.cnt) * pl.rep - sh.q0));
+    const int d = 4 * lane;
+#pragma unroll 2
+    for (int q = qg + warp; q < last; q += kJoinWarps) {
+        float M = -INFINITY;
+        for (int i = sh.i0 + lane; i <= sh.i1; i += 32) M = fmaxf(M, slot_ml<DP>(p.ws, tile, G, sh.slot(i))[q].x);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float ref = M == -INFINITY ? 0.f : M;
+        float L = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = sh.i0; i <= sh.i1; ++i) {
+            const int s = sh.slot(i);
+            const float2 ml = slot_ml<DP>(p.ws, tile, G, s)[q];
+            const float f = ex2((ml.x - ref) * U);
+            L = fmaf(ml.y, f, L);
+            if (d < D) {
+                const float4 v = *reinterpret_cast<const float4 *>(slot_o<DP>(p.ws, tile, s) + static_cast<int64_t>(q) * DP + d);
+                y.x = fmaf(v.x, f, y.x);
+                y.y = fmaf(v.y, f, y.y);
+                y.z = fmaf(v.z, f, y.z);
+                y.w = fmaf(v.w, f, y.w);
+            }
+        }
+        const int64_t qr = sh.q0 + q;
+        const int tok = static_cast<int>(div64(qr, pl.rep)), hq = h * pl.rep + static_cast<int>(qr - static_cast<int64_t>(tok) * pl.rep);
+        float so;
+        const float f = out_factor<MASK>(M, L, p.sinks, hq, so) * so;
+        if (d < D)
+            store4<BF16>(p.out, (static_cast<int64_t>(sh.b) * p.r.T + tok) * p.ldo + static_cast<int64_t>(hq) * D + d,
+                         make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
+    }
+}
+
 // ---------------------------------------------------------------- host side
 int device_sms() {
     static const int n = [] {
@@ -611,13 +648,13 @@ bool code_map(CUtensorMap &map, const Kv8Cache &c, int8_t *codes, int DP, int ro
 }
 
 // after a split kernel of G CTAs over units of `unit` rows and tiles of `tile` queries
-template <int DP, bool BF16, bool MASK>
+template <int DP, bool BF16, bool MASK, bool ROWS>
 cudaError_t join_launch(const Kv8AttnParams &p, int G, int tile, int unit, cudaStream_t s) {
     const int64_t tiles = (static_cast<int64_t>(p.r.T) * (p.Hq / p.c.Hkv) + tile - 1) / tile;
-    const int64_t joins = tiles * p.c.B * p.c.Hkv * tile;
+    const int64_t joins = tiles * p.c.B * p.c.Hkv * (ROWS ? tile / kJoinRows : tile);
     if (joins > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    return launch_pdl(kv8_attn_join_kernel<DP, BF16, MASK>, dim3(static_cast<unsigned>(joins)), dim3(kJoinWarps * 32), 0, s, p,
-                      G, tile, unit);
+    return launch_pdl(ROWS ? kv8_attn_join_rows_kernel<DP, BF16, MASK> : kv8_attn_join_kernel<DP, BF16, MASK>,
+                      dim3(static_cast<unsigned>(joins)), dim3(kJoinWarps * 32), 0, s, p, G, tile, unit);
 }
 
 template <int DP, int NT, bool BF16, bool MASK>
@@ -646,7 +683,7 @@ struct Split {
         const cudaError_t e = launch_pdl(kv8_attn_split_kernel<DP, NT, BF16, MASK, R, NS>, dim3(G), dim3(kWarps * 32), smem, s,
                                          mk, mv, p);
         if (e != cudaSuccess) return e;
-        return join_launch<DP, BF16, MASK>(p, G, 8 * NT, kWarps * 16 * R, s);
+        return join_launch<DP, BF16, MASK, false>(p, G, 8 * NT, kWarps * 16 * R, s);
     }
 };
 
@@ -702,8 +739,8 @@ cudaError_t kv8_attn_launch(const Kv8AttnParams &p, bool bf16, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const auto join = [&](auto dp) {
         constexpr int DP = decltype(dp)::value;
-        if (bf16) return p.mask ? join_launch<DP, true, true>(p, G, tile, unit, s) : join_launch<DP, true, false>(p, G, tile, unit, s);
-        return p.mask ? join_launch<DP, false, true>(p, G, tile, unit, s) : join_launch<DP, false, false>(p, G, tile, unit, s);
+        if (bf16) return p.mask ? join_launch<DP, true, true, true>(p, G, tile, unit, s) : join_launch<DP, true, false, true>(p, G, tile, unit, s);
+        return p.mask ? join_launch<DP, false, true, true>(p, G, tile, unit, s) : join_launch<DP, false, false, true>(p, G, tile, unit, s);
     };
     return p.c.D <= 64 ? join(std::integral_constant<int, 64>{}) : join(std::integral_constant<int, 128>{});
 }

@@ -10,8 +10,9 @@
 //
 // One CTA per SM walks its part of the list of units (128 rows of one tile and kv head; Walk). Warp roles:
 //  * softmax warps (four per query tile; a thread is a query): stage the tile's queries, then per row tile read S,
-//    form the weights, write P; at a segment's end scale O and store it (or a partial). Scores are read once: the
-//    reference m is that of the tiles before, and only if a score passes it by too much is the tile done again.
+//    form the weights, write P; at a segment's end scale O and store it (or a partial). S is read twice, for the
+//    largest score and for the weights, 32 columns at a time: holding the weights back instead, until the reference is
+//    known to stand, spilled, and its unrolled code missed the instruction cache (412 -> XXX us).
 //  * four decode warps: 128 rows of codes, K and V in turn, from memory (the next tile's loads in flight) to fp16 in
 //    the 128-byte-swizzled layout, two stages each. K is read K-major, V (rows are K of the product) MN-major.
 //  * one warp issues the products and owns tensor memory.
@@ -35,12 +36,13 @@ namespace {
 constexpr int kRows = 128;                               // rows of a tile, queries of a tile
 constexpr int kSub = kRows * 128;                        // bytes of 128 rows x 64 fp16
 constexpr int kBars = 20;
+constexpr int kDec = 4;                                  // decode warps
 
 template <int DP, int QT, int PARTS>
 struct TileSizes {
     static constexpr int tile = kRows * DP * 2;          // 128 rows of DP fp16: DP / 64 sub-tiles of 64
     static constexpr int smem = 1024 + (QT * PARTS + 4) * tile + kBars * 8 + 16;
-    static constexpr int soft = 4 * QT, threads = (soft + 5) * 32;
+    static constexpr int soft = 4 * QT, threads = (soft + kDec + 1) * 32;
 };
 
 // byte offset of 16-byte chunk c (8 fp16) of row r in a tile
@@ -49,6 +51,28 @@ __device__ __forceinline__ uint32_t tile_off(int r, int c) {
 }
 __device__ __forceinline__ void sts_v4(uint32_t addr, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// pairs of fp32 in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
 }
 // instruction descriptor: fp32 accumulator, fp16 A and B, B MN-major or K-major, N x 128
 template <int N, bool BMN>
@@ -60,7 +84,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
     using Z = TileSizes<DP, QT, PARTS>;
     constexpr int CH = DP / 16;                          // 16-code chunks of a row
     constexpr float U = MASK ? kLog2e : 1.f, RAISE = MASK ? 4.f : 6.f;
-    constexpr int kO = 256;                              // tensor-memory column of O; S buffers at 0 and 128
+    constexpr int kO = 256, kP2 = kO + 128;              // tensor-memory columns of O, of the weights' second parts; S at 0, 128
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t qs = base, ks = qs + QT * PARTS * Z::tile, vs = ks + 2 * Z::tile, bars = vs + 2 * Z::tile;
@@ -76,9 +100,9 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
             mbar_init(s_full + 8 * i, 1);                // commits
             mbar_init(p_full + 8 * i, 4);
             mbar_init(o_full + 8 * i, 1);
-            mbar_init(k_full + 8 * i, 4);                // decode warps
+            mbar_init(k_full + 8 * i, kDec);             // decode warps
             mbar_init(k_empty + 8 * i, 1);
-            mbar_init(v_full + 8 * i, 4);
+            mbar_init(v_full + 8 * i, kDec);
             mbar_init(v_empty + 8 * i, 1);
         }
         mbar_init(drain, 1);
@@ -86,7 +110,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
     }
     pdl_wait_prerequisites();
     pdl_launch_dependents();                             // after the wait: the join may read pos and cnt as it starts
-    if (warp == Z::soft + 4) {
+    if (warp == Z::soft + kDec) {
         tmem_alloc(slot_addr, 512);
         tmem_relinquish();
     }
@@ -211,76 +235,47 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
                     }
                     bool touch = fix != 1.f;                     // uniform
                     const bool edged = MASK || r0 + kRows > edge;
-                    uint32_t ph[64], pw[PARTS == 2 ? 64 : 1];
-                    float lt;
-                    for (int pass = 0;; ++pass) {
-                        float top = -INFINITY;
-                        lt = 0.f;
+                    // a score of the tile's column, -inf where it is not seen
+                    auto score = [&](uint32_t s, float f, int col) {
+                        float x = __uint_as_float(s) * f;
+                        if (col > lim) return -INFINITY;
+                        if constexpr (MASK) {
+                            const float mk = mrow[col];
+                            x = mk == -INFINITY ? -INFINITY : x + mk;
+                        }
+                        return x;
+                    };
+                    // the tile's largest score against the reference
+                    float top = -INFINITY;
+#pragma unroll 1
+                    for (int ch = 0; ch < 4; ++ch) {
+                        uint32_t s[32];
+                        tc_ld_32x32b_x32(stm + 32 * ch, s);
 #pragma unroll
-                        for (int ch = 0; ch < 4; ++ch) {
-                            uint32_t s[32];
-                            tc_ld_32x32b_x32(stm + 32 * ch, s);
+                        for (int g = 0; g < 2; ++g) {
+                            const float f = rs * __shfl_sync(0xffffffffu, scj, 2 * ch + g);
+                            if (!edged) {                        // scales are not negative
+                                float t = __uint_as_float(s[16 * g]);
 #pragma unroll
-                            for (int g = 0; g < 2; ++g) {
-                                const float f = rs * __shfl_sync(0xffffffffu, scj, 2 * ch + g);
-                                const float wv = cv * __shfl_sync(0xffffffffu, scj, 8 + 2 * ch + g);
-                                if (!edged) {
+                                for (int k = 1; k < 16; ++k) t = fmaxf(t, __uint_as_float(s[16 * g + k]));
+                                top = fmaxf(top, t * f);
+                            } else {
 #pragma unroll
-                                    for (int k = 0; k < 16; k += 2) {
-                                        const float a0 = fmaf(__uint_as_float(s[16 * g + k]), f, -m);
-                                        const float a1 = fmaf(__uint_as_float(s[16 * g + k + 1]), f, -m);
-                                        top = fmaxf(top, fmaxf(a0, a1));
-                                        const float e0 = ex2(a0 * U), e1 = ex2(a1 * U);
-                                        lt += e0 + e1;
-                                        const float w0 = e0 * wv, w1 = e1 * wv;
-                                        ph[16 * ch + 8 * g + k / 2] = pack_h2(w0, w1);
-                                        if constexpr (PARTS == 2) {
-                                            const float2 r = unpack_h2(ph[16 * ch + 8 * g + k / 2]);
-                                            pw[16 * ch + 8 * g + k / 2] = pack_h2(w0 - r.x, w1 - r.y);
-                                        }
-                                    }
-                                } else {
-#pragma unroll
-                                    for (int k = 0; k < 16; k += 2) {
-                                        float w2[2];
-#pragma unroll
-                                        for (int i = 0; i < 2; ++i) {
-                                            const int col = r0 + 32 * ch + 16 * g + k + i;
-                                            float x = __uint_as_float(s[16 * g + k + i]) * f;
-                                            bool seen = col <= lim;
-                                            if constexpr (MASK) {
-                                                const float mk = seen ? mrow[col] : -INFINITY;
-                                                seen = mk != -INFINITY;
-                                                x += mk;
-                                            }
-                                            const float a = seen ? x - m : -INFINITY;
-                                            top = fmaxf(top, a);
-                                            const float e = ex2(a * U);
-                                            lt += e;
-                                            // a row that is not seen weighs nothing, even where its scale is NaN
-                                            w2[i] = a == -INFINITY ? 0.f : e * wv;
-                                        }
-                                        ph[16 * ch + 8 * g + k / 2] = pack_h2(w2[0], w2[1]);
-                                        if constexpr (PARTS == 2) {
-                                            const float2 r = unpack_h2(ph[16 * ch + 8 * g + k / 2]);
-                                            pw[16 * ch + 8 * g + k / 2] = pack_h2(w2[0] - r.x, w2[1] - r.y);
-                                        }
-                                    }
-                                }
+                                for (int k = 0; k < 16; ++k) top = fmaxf(top, score(s[16 * g + k], f, r0 + 32 * ch + 16 * g + k));
                             }
                         }
-                        const bool raise = top > RAISE || (!have && top > -INFINITY);
-                        if (pass == 1 || !__any_sync(0xffffffffu, raise)) break;
+                    }
+                    const bool raise = top > m + RAISE || (!have && top > -INFINITY);
+                    if (__any_sync(0xffffffffu, raise)) {
                         if (raise) {
-                            const float a = have ? ex2(-top * U) : 0.f;
-                            m += top;
+                            const float a = have ? ex2((m - top) * U) : 0.f;
+                            m = top;
                             l *= a;
                             fix *= a;
                             have = true;
                         }
                         touch = true;
                     }
-                    l += lt;
                     if (touch && j > 0) {                        // O onto the new reference, once its last product is done
                         if (!failed)
                             failed = __any_sync(0xffffffffu, !mbar_wait_bounded(o_full + 8 * qt, (pv - 1) & 1, kWaitNs));
@@ -294,12 +289,50 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
                             tc_st_32x32b_x32(otm + 32 * ch, v);
                         }
                     }
-                    tc_st_32x32b_x32(stm, ph);
-                    tc_st_32x32b_x32(stm + 32, ph + 32);
-                    if constexpr (PARTS == 2) {
-                        tc_st_32x32b_x32(stm + 64, pw);
-                        tc_st_32x32b_x32(stm + 96, pw + 32);
+                    // weights: 32 scores at a time, their pairs over the first half of the columns read so far (the second
+                    // parts of fp32 calls in a buffer of their own)
+                    const float2 mm = make_float2(-m, -m);
+                    float2 lt = make_float2(0.f, 0.f);
+#pragma unroll 1
+                    for (int ch = 0; ch < 4; ++ch) {
+                        uint32_t s[32], ph[16], pw[16];
+                        tc_ld_32x32b_x32(stm + 32 * ch, s);
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            const float f = rs * __shfl_sync(0xffffffffu, scj, 2 * ch + g);
+                            const float wv = cv * __shfl_sync(0xffffffffu, scj, 8 + 2 * ch + g);
+                            auto keep = [&](int k, float2 w) {
+                                ph[8 * g + k / 2] = pack_h2(w.x, w.y);
+                                if constexpr (PARTS == 2) {
+                                    const float2 r = unpack_h2(ph[8 * g + k / 2]);
+                                    pw[8 * g + k / 2] = pack_h2(w.x - r.x, w.y - r.y);
+                                }
+                            };
+                            if (!edged) {
+#pragma unroll
+                                for (int k = 0; k < 16; k += 2) {
+                                    const float2 a = fma2(make_float2(__uint_as_float(s[16 * g + k]), __uint_as_float(s[16 * g + k + 1])),
+                                                          make_float2(f, f), mm);
+                                    const float2 e = make_float2(ex2(a.x * U), ex2(a.y * U));
+                                    lt = add2(lt, e);
+                                    keep(k, mul2(e, make_float2(wv, wv)));
+                                }
+                            } else {
+#pragma unroll
+                                for (int k = 0; k < 16; k += 2) {
+                                    const int col = r0 + 32 * ch + 16 * g + k;
+                                    const float x0 = score(s[16 * g + k], f, col), x1 = score(s[16 * g + k + 1], f, col + 1);
+                                    const float2 e = make_float2(ex2((x0 - m) * U), ex2((x1 - m) * U));
+                                    lt = add2(lt, e);
+                                    // a row that is not seen weighs nothing, even where its scale is NaN
+                                    keep(k, make_float2(x0 == -INFINITY ? 0.f : e.x * wv, x1 == -INFINITY ? 0.f : e.y * wv));
+                                }
+                            }
+                        }
+                        tc_st_32x32b_x16(stm + 16 * ch, ph);
+                        if constexpr (PARTS == 2) tc_st_32x32b_x16(tmem + lanes + kP2 + 64 * buf + 16 * ch, pw);
                     }
+                    l += lt.x + lt.y;
                     tc_wait_st();
                 }
                 tc_fence_before();
@@ -336,25 +369,27 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
             tc_fence_before();
             __syncwarp();
         }
-    } else if (warp < Z::soft + 4) {
+    } else if (warp < Z::soft + kDec) {
         // ============================================================ decode
         const int dt = threadIdx.x - Z::soft * 32;
         for (; wk.segment(p, pl); wk.next()) {
             const int row0 = wk.ua * kRows, row1 = min(wk.len, wk.ub * kRows), n = wk.ub - wk.ua;
             const int8_t *kb = c.k + wk.b * c.bs + wk.h * c.hs, *vb = c.v + wk.b * c.bs + wk.h * c.hs;
-            // a thread's chunks of a tile: chunk dt % CH of rows dt / CH + i * 128 / CH
-            auto load = [&](const int8_t *src, int r0, uint4 (&x)[CH]) {
+            // a thread's chunks of a tile: every (32 kDec)-th, CH chunks to a row
+            constexpr int IT = (kRows * CH + 32 * kDec - 1) / (32 * kDec);
+            auto load = [&](const int8_t *src, int r0, uint4 (&x)[IT]) {
 #pragma unroll
-                for (int i = 0; i < CH; ++i) {
-                    const int r = r0 + dt / CH + i * (kRows / CH), ch = dt % CH;
-                    x[i] = r < row1 && ch * 16 < D ? ld_nc_v4(src + static_cast<int64_t>(r) * c.rs + ch * 16)
-                                                   : make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < IT; ++i) {
+                    const int idx = dt + i * 32 * kDec, r = r0 + idx / CH, ch = idx % CH;
+                    x[i] = r < row1 && idx < kRows * CH && ch * 16 < D
+                               ? ld_nc_v4(src + static_cast<int64_t>(r) * c.rs + ch * 16) : make_uint4(0, 0, 0, 0);
                 }
             };
-            auto store = [&](uint32_t dst, const uint4 (&x)[CH]) {
+            auto store = [&](uint32_t dst, const uint4 (&x)[IT]) {
 #pragma unroll
-                for (int i = 0; i < CH; ++i) {
-                    const int r = dt / CH + i * (kRows / CH), ch = dt % CH;
+                for (int i = 0; i < IT; ++i) {
+                    const int idx = dt + i * 32 * kDec, r = idx / CH, ch = idx % CH;
+                    if (idx >= kRows * CH) break;
                     const uint32_t w[4] = {x[i].x ^ 0x80808080u, x[i].y ^ 0x80808080u, x[i].z ^ 0x80808080u, x[i].w ^ 0x80808080u};
                     const uint4 lo = make_uint4(h2_lo(w[0]), h2_hi(w[0]), h2_lo(w[1]), h2_hi(w[1]));
                     const uint4 hi = make_uint4(h2_lo(w[2]), h2_hi(w[2]), h2_lo(w[3]), h2_hi(w[3]));
@@ -363,7 +398,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
                     sts_v4(dst + tile_off(r, 2 * ch + 1 - odd), odd ? lo : hi);
                 }
             };
-            uint4 xk[CH], xv[CH];
+            uint4 xk[IT], xv[IT];
             load(kb, row0, xk);
             for (int j = 0; j < n; ++j, ++jt) {
                 const int st = jt & 1, use = jt >> 1;
@@ -406,7 +441,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
                 for (int pt = 0; pt < PARTS; ++pt)
 #pragma unroll
                     for (int kk = 0; kk < kRows / 16; ++kk)
-                        tc_mma_f16_ta(tmem + kO + qt * DP, tmem + buf * kRows + pt * 64 + kk * 8,
+                        tc_mma_f16_ta(tmem + kO + qt * DP, tmem + (pt ? kP2 + buf * 64 : buf * kRows) + kk * 8,
                                       sw128_desc_mn(vs + (tile & 1) * Z::tile + kk * 2048, kSub), kIdesc<DP, true>,
                                       more || (pt | kk) != 0);
             }
@@ -447,7 +482,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
     if (failed && lane == 0) atomicOr(p.r.err, 64);
     tc_fence_before();
     __syncthreads();
-    if (warp == Z::soft + 4) tmem_dealloc(tmem, 512);
+    if (warp == Z::soft + kDec) tmem_dealloc(tmem, 512);
 }
 
 int sms() {
