@@ -8,6 +8,7 @@
 #include <cstdint>
 
 #include "kernels.h"
+#include "tmap.h"
 
 namespace onpu_b200 {
 
@@ -237,6 +238,23 @@ __device__ __forceinline__ float out_factor(float M, float Lsum, const float *si
         total = Lsum * scale_o + ex2((sk - ref) * U);
     }
     return total == 0.f ? 0.f : 1.f / total;
+}
+
+// (host) a map of [batch][heads][rows][dim] codes whose boxes are `rows` rows of at most 128 codes, their 16-byte
+// chunks exchanged by `swizzle`; columns and rows past the ends read 0
+inline bool kv8_code_map(CUtensorMap &map, const Kv8Cache &c, int8_t *codes, int DP, int rows, CUtensorMapSwizzle swizzle) {
+    const auto fn = tensor_map_encode_fn();
+    if (!fn) return false;
+    const cuuint32_t box[4] = {static_cast<cuuint32_t>(DP < 128 ? DP : 128), static_cast<cuuint32_t>(rows), 1, 1};
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.D), static_cast<cuuint64_t>(c.S), static_cast<cuuint64_t>(c.Hkv),
+                                static_cast<cuuint64_t>(c.B)};
+    // a lone head's or sequence's stride is not used: any valid one
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(c.rs), static_cast<cuuint64_t>(c.Hkv > 1 ? c.hs : c.rs),
+                                   static_cast<cuuint64_t>(c.B > 1 ? c.bs : c.rs)};
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    return fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, codes, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace onpu_b200

@@ -35,7 +35,6 @@
 #include "kernels.h"
 #include "kv8.cuh"
 #include "ptx.cuh"
-#include "tmap.h"
 
 namespace onpu_b200 {
 namespace {
@@ -630,23 +629,6 @@ constexpr int kTileFrom = 16;
 bool use_tiles(int D, int64_t queries) { return D <= 128 && queries > kTileFrom; }
 int padded_dim(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
-// a map of [batch][heads][rows][dim] codes whose boxes are `rows` rows of at most 128 codes, chunks exchanged
-// within a row; columns and rows past the ends read 0
-bool code_map(CUtensorMap &map, const Kv8Cache &c, int8_t *codes, int DP, int rows) {
-    const auto fn = tensor_map_encode_fn();
-    if (!fn) return false;
-    const cuuint32_t box[4] = {static_cast<cuuint32_t>(DP < 128 ? DP : 128), static_cast<cuuint32_t>(rows), 1, 1};
-    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.D), static_cast<cuuint64_t>(c.S), static_cast<cuuint64_t>(c.Hkv),
-                                static_cast<cuuint64_t>(c.B)};
-    // a lone head's or sequence's stride is not used: any valid one
-    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(c.rs), static_cast<cuuint64_t>(c.Hkv > 1 ? c.hs : c.rs),
-                                   static_cast<cuuint64_t>(c.B > 1 ? c.bs : c.rs)};
-    const cuuint32_t ones[4] = {1, 1, 1, 1};
-    return fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, codes, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              DP == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 // after a split kernel of G CTAs over units of `unit` rows and tiles of `tile` queries
 template <int DP, bool BF16, bool MASK, bool ROWS>
 cudaError_t join_launch(const Kv8AttnParams &p, int G, int tile, int unit, cudaStream_t s) {
@@ -679,7 +661,9 @@ struct Split {
         const int64_t tiles = (static_cast<int64_t>(p.r.T) * rep + 8 * NT - 1) / (8 * NT);
         if (tiles * p.c.B > 0x7fffffff) return cudaErrorInvalidConfiguration;
         CUtensorMap mk, mv;
-        if (!code_map(mk, p.c, p.c.k, DP, 16 * R) || !code_map(mv, p.c, p.c.v, DP, 16 * R)) return cudaErrorInvalidValue;
+        const auto swz = DP == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+        if (!kv8_code_map(mk, p.c, p.c.k, DP, 16 * R, swz) || !kv8_code_map(mv, p.c, p.c.v, DP, 16 * R, swz))
+            return cudaErrorInvalidValue;
         const cudaError_t e = launch_pdl(kv8_attn_split_kernel<DP, NT, BF16, MASK, R, NS>, dim3(G), dim3(kWarps * 32), smem, s,
                                          mk, mv, p);
         if (e != cudaSuccess) return e;

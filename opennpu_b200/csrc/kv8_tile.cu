@@ -9,12 +9,12 @@
 // calls: two parts), m raised only when a score passes it by 2^6 (e^4 with a mask, scores then in natural units).
 //
 // One CTA per SM walks its part of the list of units (128 rows of one tile and kv head; Walk). Warp roles:
-//  * softmax warps (four per query tile; a thread is a query): stage the tile's queries, then per row tile read S,
-//    form the weights, write P; at a segment's end scale O and store it (or a partial). S is read twice, for the
-//    largest score and for the weights, 32 columns at a time: holding the weights back instead, until the reference is
-//    known to stand, spilled, and its unrolled code missed the instruction cache (412 -> XXX us).
-//  * four decode warps: 128 rows of codes, K and V in turn, from memory (the next tile's loads in flight) to fp16 in
-//    the 128-byte-swizzled layout, two stages each. K is read K-major, V (rows are K of the product) MN-major.
+//  * softmax warps, eight per query tile: a thread is a query and one half of a row tile's columns, so that the time
+//    from scores to weights, which the products wait for, is half as long. Per row tile: the largest score (a barrier with
+//    a vote joins the halves; the reference m is raised only if one asks), then the weights, 32 at a time, written over the
+//    scores just read. At a segment's end O is scaled and stored (or a partial).
+//  * three decode warps: codes that TMA brought (128 rows, K and V in turn, one of each ahead) to fp16 in the
+//    128-byte-swizzled layout, two stages each. K is read K-major, V (rows are K of the product) MN-major.
 //  * one warp issues the products and owns tensor memory.
 // QT = 2 query tiles share a decoded row tile and alternate: one's softmax runs beside the other's products. QT = 1
 // (at most 128 queries, or fp32) alternates two S buffers instead.
@@ -29,20 +29,24 @@
 #include "kv8.cuh"
 #include "ptx.cuh"
 #include "tc.cuh"
+#include "tmap.h"
 
 namespace onpu_b200 {
 namespace {
 
 constexpr int kRows = 128;                               // rows of a tile, queries of a tile
 constexpr int kSub = kRows * 128;                        // bytes of 128 rows x 64 fp16
-constexpr int kBars = 20;
-constexpr int kDec = 4;                                  // decode warps
+constexpr int kBars = 24;
+constexpr int kDec = 3;                                  // decode warps: 12 or 20 warps in all, 3 or 5 a scheduler
 
 template <int DP, int QT, int PARTS>
 struct TileSizes {
     static constexpr int tile = kRows * DP * 2;          // 128 rows of DP fp16: DP / 64 sub-tiles of 64
-    static constexpr int smem = 1024 + (QT * PARTS + 4) * tile + kBars * 8 + 16;
-    static constexpr int soft = 4 * QT, threads = (soft + kDec + 1) * 32;
+    static constexpr int raw = kRows * DP;               // 128 rows of codes
+    static constexpr int share = QT * 2 * kRows * 4;     // a float per softmax thread
+    static constexpr int smem = (QT * PARTS + 4) * tile + 2 * raw + share + kBars * 8 + 16;
+    static_assert(smem <= 227 * 1024, "a CTA's shared memory");
+    static constexpr int soft = 8 * QT, threads = (soft + kDec + 1) * 32;
 };
 
 // byte offset of 16-byte chunk c (8 fp16) of row r in a tile
@@ -52,26 +56,9 @@ __device__ __forceinline__ uint32_t tile_off(int r, int c) {
 __device__ __forceinline__ void sts_v4(uint32_t addr, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-// pairs of fp32 in one instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
-        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-        "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-        "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 // instruction descriptor: fp32 accumulator, fp16 A and B, B MN-major or K-major, N x 128
@@ -79,31 +66,54 @@ template <int N, bool BMN>
 constexpr uint32_t kIdesc = (1u << 4) | (BMN ? 1u << 16 : 0u) | (static_cast<uint32_t>(N >> 3) << 17) |
                             (static_cast<uint32_t>(kRows >> 4) << 24);
 
+// whether any of the barrier's threads votes yes
+__device__ __forceinline__ bool bar_any(int id, int count, bool vote) {
+    int r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %3, 0;\n\t"
+        "barrier.cta.red.or.pred q, %1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(id), "r"(count), "r"(static_cast<int>(vote))
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void tma_codes(uint32_t dst, const CUtensorMap *map, int row, int head, int seq, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        ::"r"(dst), "l"(map), "r"(0), "r"(row), "r"(head), "r"(seq), "r"(bar)
+        : "memory");
+}
+
 template <int DP, int QT, int PARTS, bool BF16, bool MASK>
-__global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn_tile_kernel(const Kv8AttnParams p) {
+__global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
+    kv8_attn_tile_kernel(const __grid_constant__ CUtensorMap mapk, const __grid_constant__ CUtensorMap mapv,
+                         const Kv8AttnParams p) {
     using Z = TileSizes<DP, QT, PARTS>;
     constexpr int CH = DP / 16;                          // 16-code chunks of a row
     constexpr float U = MASK ? kLog2e : 1.f, RAISE = MASK ? 4.f : 6.f;
     constexpr int kO = 256, kP2 = kO + 128;              // tensor-memory columns of O, of the weights' second parts; S at 0, 128
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t qs = base, ks = qs + QT * PARTS * Z::tile, vs = ks + 2 * Z::tile, bars = vs + 2 * Z::tile;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];        // the swizzle's period
+    const uint32_t base = smem_u32(smem_raw);
+    const uint32_t qs = base, ks = qs + QT * PARTS * Z::tile, vs = ks + 2 * Z::tile, raw = vs + 2 * Z::tile;
+    float *share = reinterpret_cast<float *>(smem_raw + (raw + 2 * Z::raw - smem_u32(smem_raw)));     // [QT][2][128]
+    const uint32_t bars = raw + 2 * Z::raw + Z::share;
     const uint32_t q_full = bars, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16, k_full = o_full + 16,
-                   k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16, drain = v_empty + 16;
+                   k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16, raw_full = v_empty + 16, drain = raw_full + 16;
     const uint32_t slot_addr = bars + kBars * 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = gridDim.x, D = p.c.D;
     const Kv8Cache &c = p.c;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(q_full + 8 * i, 4);                // a query tile's softmax warps
+            mbar_init(q_full + 8 * i, 8);                // a query tile's softmax warps
             mbar_init(s_full + 8 * i, 1);                // commits
-            mbar_init(p_full + 8 * i, 4);
+            mbar_init(p_full + 8 * i, 8);
             mbar_init(o_full + 8 * i, 1);
-            mbar_init(k_full + 8 * i, kDec);             // decode warps
+            mbar_init(k_full + 8 * i, 1);                // a decode thread, for all
             mbar_init(k_empty + 8 * i, 1);
-            mbar_init(v_full + 8 * i, kDec);
+            mbar_init(v_full + 8 * i, 1);
             mbar_init(v_empty + 8 * i, 1);
+            mbar_init(raw_full + 8 * i, 1);              // copies
         }
         mbar_init(drain, 1);
         mbar_init_fence();
@@ -129,7 +139,8 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
         // nothing for this CTA
     } else if (warp < Z::soft) {
         // ============================================================ softmax
-        const int qt = warp >> 2, row = (warp & 3) * 32 + lane;
+        const int qt = warp >> 3, hf = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
+        float *mine = share + (qt * 2 + hf) * kRows + row, *other = share + (qt * 2 + (hf ^ 1)) * kRows + row;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t otm = tmem + lanes + kO + qt * DP;
         int pv = 0;                                      // products of this query tile with V so far
@@ -185,7 +196,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
             }
             const float fq = pow2_to(mx, 8), fs = p.scale < 0.f ? -fq : fq;     // a negative scale: on the query
 #pragma unroll 4
-            for (int d = 0; d < DP; d += 8) {
+            for (int d = hf * (DP / 2); d < (hf + 1) * (DP / 2); d += 8) {      // each thread its half of the row
                 float x[8];
                 load8(d, x);
                 uint32_t w[4], w2[4];
@@ -222,117 +233,135 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
                 if (!failed) failed = __any_sync(0xffffffffu, !mbar_wait_bounded(s_full + 8 * buf, sphase, kWaitNs));
                 ++ns;
                 tc_fence_after();
-                if (edge > 0) {                                  // a warp without a valid query leaves its lanes of P as they are
-                    // V's largest scale (bits: NaN does not count) against the weights' power of two
-                    uint32_t vb = lane >= 8 && lane < 16 ? __float_as_uint(scj) : 0u;
-                    vb = __reduce_max_sync(0xffffffffu, vb <= 0x7f800000u ? vb : 0u);
-                    const float vmax = __uint_as_float(vb);
-                    float fix = 1.f;                             // of O, for a new power of two and a new reference
-                    if (vmax * cv > 512.f || (cv == 0.f && vmax > 0.f)) {
-                        const float cn = pow2_to(vmax, 7);
-                        if (cv != 0.f) fix = cn / cv;
-                        cv = cn;
-                    }
-                    bool touch = fix != 1.f;                     // uniform
-                    const bool edged = MASK || r0 + kRows > edge;
-                    // a score of the tile's column, -inf where it is not seen
-                    auto score = [&](uint32_t s, float f, int col) {
-                        float x = __uint_as_float(s) * f;
-                        if (col > lim) return -INFINITY;
-                        if constexpr (MASK) {
-                            const float mk = mrow[col];
-                            x = mk == -INFINITY ? -INFINITY : x + mk;
-                        }
-                        return x;
-                    };
-                    // the tile's largest score against the reference
-                    float top = -INFINITY;
+                const bool live = edge > 0;                      // a warp without a valid query leaves its lanes of P as they are
+                // V's largest scale (bits: NaN does not count) against the weights' power of two
+                uint32_t vb = lane >= 8 && lane < 16 ? __float_as_uint(scj) : 0u;
+                vb = __reduce_max_sync(0xffffffffu, vb <= 0x7f800000u ? vb : 0u);
+                const float vmax = __uint_as_float(vb);
+                // O times a, once its last product is done: this half of its columns
+                const auto rescale_o = [&](float a) {
+                    if (j == 0 || !live) return;                 // O begins with this tile
+                    if (!failed)
+                        failed = __any_sync(0xffffffffu, !mbar_wait_bounded(o_full + 8 * qt, (pv - 1) & 1, kWaitNs));
+                    tc_fence_after();
 #pragma unroll 1
-                    for (int ch = 0; ch < 4; ++ch) {
+                    for (int ch = hf * (DP / 32); ch < (hf + 1) * (DP / 32); ++ch) {
+                        uint32_t v[16];
+                        tc_ld_32x32b_x16(otm + 16 * ch, v);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * a);
+                        tc_st_32x32b_x16(otm + 16 * ch, v);
+                    }
+                };
+                if (vmax * cv > 512.f || (cv == 0.f && vmax > 0.f)) {
+                    const float cn = pow2_to(vmax, 7);
+                    if (cv != 0.f) rescale_o(cn / cv);
+                    cv = cn;
+                }
+                const float vv = cv * scj, lg = __log2f(vv), rv = 1.f / vv;
+                const auto scale_k = [&](int g) { return rs * __shfl_sync(0xffffffffu, scj, g); };
+                const bool above0 = !(lane >= 8 && lane < 16 && !(scj > 0.f));
+                const bool usual = !MASK && r0 + kRows <= edge && __all_sync(0xffffffffu, above0);
+                // a finished score of the tile's column, -inf where it is not seen
+                const auto score = [&](uint32_t s, float f, int col) {
+                    const float x = __uint_as_float(s) * f;
+                    if constexpr (MASK) {
+                        const float mk = col <= lim ? mrow[col] : -INFINITY;
+                        return mk == -INFINITY ? -INFINITY : x + mk;
+                    }
+                    return col <= lim ? x : -INFINITY;
+                };
+                // the largest score of this half
+                float top = -INFINITY;
+                if (live) {
+#pragma unroll 1
+                    for (int ch = 2 * hf; ch < 2 * hf + 2; ++ch) {
                         uint32_t s[32];
-                        tc_ld_32x32b_x32(stm + 32 * ch, s);
+                        tc_ld_issue_x32(stm + 32 * ch, s);
+                        tc_wait_ld32(s);
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
-                            const float f = rs * __shfl_sync(0xffffffffu, scj, 2 * ch + g);
-                            if (!edged) {                        // scales are not negative
-                                float t = __uint_as_float(s[16 * g]);
+                            const float f = scale_k(2 * ch + g);
+                            if (usual) {                         // scales are not negative
+                                float t0 = __uint_as_float(s[16 * g]), t1 = __uint_as_float(s[16 * g + 1]);
 #pragma unroll
-                                for (int k = 1; k < 16; ++k) t = fmaxf(t, __uint_as_float(s[16 * g + k]));
-                                top = fmaxf(top, t * f);
+                                for (int k = 2; k < 14; k += 4) {
+                                    t0 = max3(t0, __uint_as_float(s[16 * g + k]), __uint_as_float(s[16 * g + k + 1]));
+                                    t1 = max3(t1, __uint_as_float(s[16 * g + k + 2]), __uint_as_float(s[16 * g + k + 3]));
+                                }
+                                t0 = max3(t0, __uint_as_float(s[16 * g + 14]), __uint_as_float(s[16 * g + 15]));
+                                top = fmaxf(top, fmaxf(t0, t1) * f);
                             } else {
 #pragma unroll
                                 for (int k = 0; k < 16; ++k) top = fmaxf(top, score(s[16 * g + k], f, r0 + 32 * ch + 16 * g + k));
                             }
                         }
                     }
-                    const bool raise = top > m + RAISE || (!have && top > -INFINITY);
-                    if (__any_sync(0xffffffffu, raise)) {
-                        if (raise) {
-                            const float a = have ? ex2((m - top) * U) : 0.f;
-                            m = top;
-                            l *= a;
-                            fix *= a;
-                            have = true;
-                        }
-                        touch = true;
+                }
+                if (bar_any(2 + qt, 256, top > m + RAISE || (!have && top > -INFINITY))) {
+                    *mine = top;
+                    named_bar_sync(2 + qt, 256);
+                    top = fmaxf(top, *other);                    // the row's, in both its threads
+                    float a = 1.f;
+                    if (top > m + RAISE || (!have && top > -INFINITY)) {
+                        a = have ? ex2((m - top) * U) : 0.f;
+                        m = top;
+                        l *= a;
+                        have = true;
                     }
-                    if (touch && j > 0) {                        // O onto the new reference, once its last product is done
-                        if (!failed)
-                            failed = __any_sync(0xffffffffu, !mbar_wait_bounded(o_full + 8 * qt, (pv - 1) & 1, kWaitNs));
-                        tc_fence_after();
+                    if (__any_sync(0xffffffffu, a != 1.f)) rescale_o(a);
+                }
+                // the weights of this half
+                if (live) {
 #pragma unroll 1
-                        for (int ch = 0; ch < DP / 32; ++ch) {
-                            uint32_t v[32];
-                            tc_ld_32x32b_x32(otm + 32 * ch, v);
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * fix);
-                            tc_st_32x32b_x32(otm + 32 * ch, v);
-                        }
-                    }
-                    // weights: 32 scores at a time, their pairs over the first half of the columns read so far (the second
-                    // parts of fp32 calls in a buffer of their own)
-                    const float2 mm = make_float2(-m, -m);
-                    float2 lt = make_float2(0.f, 0.f);
-#pragma unroll 1
-                    for (int ch = 0; ch < 4; ++ch) {
+                    for (int ch = 0; ch < 2; ++ch) {
                         uint32_t s[32], ph[16], pw[16];
-                        tc_ld_32x32b_x32(stm + 32 * ch, s);
+                        tc_ld_issue_x32(stm + 64 * hf + 32 * ch, s);
+                        tc_wait_ld32(s);
+                        const auto keep = [&](int i, float w0, float w1) {
+                            ph[i] = pack_h2(w0, w1);
+                            if constexpr (PARTS == 2) {
+                                const float2 r = unpack_h2(ph[i]);
+                                pw[i] = pack_h2(w0 - r.x, w1 - r.y);
+                            }
+                        };
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
-                            const float f = rs * __shfl_sync(0xffffffffu, scj, 2 * ch + g);
-                            const float wv = cv * __shfl_sync(0xffffffffu, scj, 8 + 2 * ch + g);
-                            auto keep = [&](int k, float2 w) {
-                                ph[8 * g + k / 2] = pack_h2(w.x, w.y);
-                                if constexpr (PARTS == 2) {
-                                    const float2 r = unpack_h2(ph[8 * g + k / 2]);
-                                    pw[8 * g + k / 2] = pack_h2(w.x - r.x, w.y - r.y);
-                                }
-                            };
-                            if (!edged) {
+                            const int gi = 4 * hf + 2 * ch + g;
+                            const float f = scale_k(gi);
+                            float s0 = 0.f, s1 = 0.f;
+                            if (usual) {
+                                // V's scales are above 0: a weight is one exponential, w = 2^(S f - m + log2(s_v c)), and the
+                                // sum takes w / (s_v c)
+                                const float at = __shfl_sync(0xffffffffu, lg, 8 + gi) - m;
 #pragma unroll
                                 for (int k = 0; k < 16; k += 2) {
-                                    const float2 a = fma2(make_float2(__uint_as_float(s[16 * g + k]), __uint_as_float(s[16 * g + k + 1])),
-                                                          make_float2(f, f), mm);
-                                    const float2 e = make_float2(ex2(a.x * U), ex2(a.y * U));
-                                    lt = add2(lt, e);
-                                    keep(k, mul2(e, make_float2(wv, wv)));
+                                    const float w0 = ex2(fmaf(__uint_as_float(s[16 * g + k]), f, at));
+                                    const float w1 = ex2(fmaf(__uint_as_float(s[16 * g + k + 1]), f, at));
+                                    s0 += w0;
+                                    s1 += w1;
+                                    keep(8 * g + k / 2, w0, w1);
                                 }
+                                l = fmaf(s0 + s1, __shfl_sync(0xffffffffu, rv, 8 + gi), l);
                             } else {
+                                const float wv = __shfl_sync(0xffffffffu, vv, 8 + gi);
+                                const int col = r0 + 64 * hf + 32 * ch + 16 * g;
 #pragma unroll
                                 for (int k = 0; k < 16; k += 2) {
-                                    const int col = r0 + 32 * ch + 16 * g + k;
-                                    const float x0 = score(s[16 * g + k], f, col), x1 = score(s[16 * g + k + 1], f, col + 1);
-                                    const float2 e = make_float2(ex2((x0 - m) * U), ex2((x1 - m) * U));
-                                    lt = add2(lt, e);
+                                    const float x0 = score(s[16 * g + k], f, col + k), x1 = score(s[16 * g + k + 1], f, col + k + 1);
+                                    const float e0 = ex2((x0 - m) * U), e1 = ex2((x1 - m) * U);
+                                    s0 += e0;
+                                    s1 += e1;
                                     // a row that is not seen weighs nothing, even where its scale is NaN
-                                    keep(k, make_float2(x0 == -INFINITY ? 0.f : e.x * wv, x1 == -INFINITY ? 0.f : e.y * wv));
+                                    keep(8 * g + k / 2, x0 == -INFINITY ? 0.f : e0 * wv, x1 == -INFINITY ? 0.f : e1 * wv);
                                 }
+                                l += s0 + s1;
                             }
                         }
-                        tc_st_32x32b_x16(stm + 16 * ch, ph);
-                        if constexpr (PARTS == 2) tc_st_32x32b_x16(tmem + lanes + kP2 + 64 * buf + 16 * ch, pw);
+                        // over this half's columns that have been read (the second parts of fp32 calls in their own)
+                        tc_st_32x32b_x16(stm + 64 * hf + 16 * ch, ph);
+                        if constexpr (PARTS == 2) tc_st_32x32b_x16(tmem + lanes + kP2 + 64 * buf + 32 * hf + 16 * ch, pw);
                     }
-                    l += lt.x + lt.y;
                     tc_wait_st();
                 }
                 tc_fence_before();
@@ -342,17 +371,21 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
             }
             if (!failed) failed = __any_sync(0xffffffffu, !mbar_wait_bounded(o_full + 8 * qt, (pv - 1) & 1, kWaitNs));
             tc_fence_after();
-            // O c^-1 relative to m: the output, or a partial
+            *mine = l;
+            named_bar_sync(2 + qt, 256);
+            l += *other;                                         // the sum of both halves
+            // O c^-1 relative to m: the output, or a partial; each half of the threads its half of the columns
             const float M = have ? m : -INFINITY, inv = cv == 0.f ? 1.f : 1.f / cv;
             float so, f = inv;
             if (wk.whole()) f = out_factor<MASK>(M, l, p.sinks, hq, so) * so * inv;
             const int64_t oo = (static_cast<int64_t>(b) * p.r.T + tok) * p.ldo + static_cast<int64_t>(hq) * D;
             float *po = slot_o<DP>(p.ws, QT * kRows, wk.slot(blockIdx.x)) + static_cast<int64_t>(qi) * DP;
 #pragma unroll 1
-            for (int ch = 0; ch < DP / 32; ++ch) {
+            for (int ch = hf * (DP / 64); ch < (hf + 1) * (DP / 64); ++ch) {
                 uint32_t v[32];
                 __syncwarp();
-                tc_ld_32x32b_x32(otm + 32 * ch, v);
+                tc_ld_issue_x32(otm + 32 * ch, v);
+                tc_wait_ld32(v);
                 if (!ok) continue;
 #pragma unroll
                 for (int k = 0; k < 32; k += 4) {
@@ -365,7 +398,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
                     }
                 }
             }
-            if (ok && !wk.whole()) slot_ml<DP>(p.ws, QT * kRows, G, wk.slot(blockIdx.x))[qi] = make_float2(M, l);
+            if (ok && hf == 0 && !wk.whole()) slot_ml<DP>(p.ws, QT * kRows, G, wk.slot(blockIdx.x))[qi] = make_float2(M, l);
             tc_fence_before();
             __syncwarp();
         }
@@ -373,49 +406,41 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
         // ============================================================ decode
         const int dt = threadIdx.x - Z::soft * 32;
         for (; wk.segment(p, pl); wk.next()) {
-            const int row0 = wk.ua * kRows, row1 = min(wk.len, wk.ub * kRows), n = wk.ub - wk.ua;
-            const int8_t *kb = c.k + wk.b * c.bs + wk.h * c.hs, *vb = c.v + wk.b * c.bs + wk.h * c.hs;
-            // a thread's chunks of a tile: every (32 kDec)-th, CH chunks to a row
-            constexpr int IT = (kRows * CH + 32 * kDec - 1) / (32 * kDec);
-            auto load = [&](const int8_t *src, int r0, uint4 (&x)[IT]) {
-#pragma unroll
-                for (int i = 0; i < IT; ++i) {
-                    const int idx = dt + i * 32 * kDec, r = r0 + idx / CH, ch = idx % CH;
-                    x[i] = r < row1 && idx < kRows * CH && ch * 16 < D
-                               ? ld_nc_v4(src + static_cast<int64_t>(r) * c.rs + ch * 16) : make_uint4(0, 0, 0, 0);
-                }
+            const int row0 = wk.ua * kRows, n = wk.ub - wk.ua;
+            const auto fetch = [&](int kv, int j) {              // codes of row tile j of K or V
+                if (dt != 0 || j >= n || failed) return;
+                const uint32_t bar = raw_full + 8 * kv;
+                mbar_arrive_expect_tx(bar, Z::raw);
+                tma_codes(raw + kv * Z::raw, kv ? &mapv : &mapk, row0 + j * kRows, wk.h, wk.b, bar);
             };
-            auto store = [&](uint32_t dst, const uint4 (&x)[IT]) {
-#pragma unroll
-                for (int i = 0; i < IT; ++i) {
-                    const int idx = dt + i * 32 * kDec, r = idx / CH, ch = idx % CH;
-                    if (idx >= kRows * CH) break;
-                    const uint32_t w[4] = {x[i].x ^ 0x80808080u, x[i].y ^ 0x80808080u, x[i].z ^ 0x80808080u, x[i].w ^ 0x80808080u};
-                    const uint4 lo = make_uint4(h2_lo(w[0]), h2_hi(w[0]), h2_lo(w[1]), h2_hi(w[1]));
-                    const uint4 hi = make_uint4(h2_lo(w[2]), h2_hi(w[2]), h2_lo(w[3]), h2_hi(w[3]));
-                    const int odd = ch >> 2 & 1;                 // the second sub-tile's halves the other way round: no bank twice
-                    sts_v4(dst + tile_off(r, 2 * ch + odd), odd ? hi : lo);
-                    sts_v4(dst + tile_off(r, 2 * ch + 1 - odd), odd ? lo : hi);
-                }
-            };
-            uint4 xk[IT], xv[IT];
-            load(kb, row0, xk);
+            fetch(0, 0);
+            fetch(1, 0);
             for (int j = 0; j < n; ++j, ++jt) {
                 const int st = jt & 1, use = jt >> 1;
-                load(vb, row0 + j * kRows, xv);
-                if (!failed && use > 0) failed = __any_sync(0xffffffffu, !mbar_wait_bounded(k_empty + 8 * st, (use - 1) & 1, kWaitNs));
-                store(ks + st * Z::tile, xk);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(k_full + 8 * st);
-                if (j + 1 < n) load(kb, row0 + (j + 1) * kRows, xk);
-                if (!failed && use > 0) failed = __any_sync(0xffffffffu, !mbar_wait_bounded(v_empty + 8 * st, (use - 1) & 1, kWaitNs));
-                store(vs + st * Z::tile, xv);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(v_full + 8 * st);
+#pragma unroll 1
+                for (int kv = 0; kv < 2; ++kv) {
+                    const uint32_t src = raw + kv * Z::raw, dst = (kv ? vs : ks) + st * Z::tile;
+                    if (!failed) failed = !mbar_wait_bounded(raw_full + 8 * kv, jt & 1, kWaitNs);
+                    if (!failed && use > 0) failed = !mbar_wait_bounded((kv ? v_empty : k_empty) + 8 * st, (use - 1) & 1, kWaitNs);
+#pragma unroll 4
+                    for (int i = dt; i < kRows * CH; i += 32 * kDec) {
+                        const int r = i / CH, ch = i % CH, odd = ch >> 2 & 1;     // odd: halves the other way round, no bank twice
+                        const uint4 x = lds_v4(src + i * 16);
+                        const uint32_t a = (odd ? x.z : x.x) ^ 0x80808080u, b = (odd ? x.w : x.y) ^ 0x80808080u;
+                        const uint32_t e = (odd ? x.x : x.z) ^ 0x80808080u, f = (odd ? x.y : x.w) ^ 0x80808080u;
+                        const uint32_t o = dst + tile_off(r, 2 * ch + odd);
+                        sts_v4(o, make_uint4(h2_lo(a), h2_hi(a), h2_lo(b), h2_hi(b)));
+                        sts_v4(o ^ 16, make_uint4(h2_lo(e), h2_hi(e), h2_lo(f), h2_hi(f)));
+                    }
+                    fence_proxy_async_smem();                    // what was stored, and that the codes have been read
+                    named_bar_sync(1, 32 * kDec);
+                    if (dt == 0) mbar_arrive((kv ? v_full : k_full) + 8 * st);
+                    fetch(kv, j + 1);
+                }
             }
         }
+        if (failed && dt == 0)                                   // copies in flight land before the CTA ends
+            for (int kv = 0; kv < 2; ++kv) mbar_wait_bounded(raw_full + 8 * kv, jt & 1, kWaitNs);
     } else if (lane == 0) {
         // ============================================================ products
         auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -441,7 +466,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1) kv8_attn
                 for (int pt = 0; pt < PARTS; ++pt)
 #pragma unroll
                     for (int kk = 0; kk < kRows / 16; ++kk)
-                        tc_mma_f16_ta(tmem + kO + qt * DP, tmem + (pt ? kP2 + buf * 64 : buf * kRows) + kk * 8,
+                        tc_mma_f16_ta(tmem + kO + qt * DP, tmem + (pt ? kP2 + buf * 64 + kk * 8 : buf * kRows + (kk >> 2) * 64 + (kk & 3) * 8),
                                       sw128_desc_mn(vs + (tile & 1) * Z::tile + kk * 2048, kSub), kIdesc<DP, true>,
                                       more || (pt | kk) != 0);
             }
@@ -502,7 +527,11 @@ cudaError_t launch_t(const Kv8AttnParams &p, cudaStream_t s) {
     const auto k = kv8_attn_tile_kernel<DP, QT, PARTS, BF16, MASK>;
     static const cudaError_t attr = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::smem);
     if (attr != cudaSuccess) return attr;
-    return launch_pdl(k, dim3(sms()), dim3(Z::threads), Z::smem, s, p);
+    CUtensorMap mk, mv;
+    if (!kv8_code_map(mk, p.c, p.c.k, DP, kRows, CU_TENSOR_MAP_SWIZZLE_NONE) ||
+        !kv8_code_map(mv, p.c, p.c.v, DP, kRows, CU_TENSOR_MAP_SWIZZLE_NONE))
+        return cudaErrorInvalidValue;
+    return launch_pdl(k, dim3(sms()), dim3(Z::threads), Z::smem, s, mk, mv, p);
 }
 template <int DP, int QT>
 cudaError_t launch_q(const Kv8AttnParams &p, bool bf16, cudaStream_t s) {
