@@ -28,6 +28,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <type_traits>
@@ -557,22 +558,22 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_kernel(const Kv
     }
 }
 
-// The same after kv8_tile.cu, whose many queries share a CTA's plan: kJoinRows queries a CTA, a warp at a time on
-// each of its share (one CTA a query took 161 us of a 512-token chunk's 450).
+// The same where a segment has few parts: up to kJoinRows queries of a tile a CTA, a warp at a time on each of its
+// share (a CTA for each query took 161 us of a 512-token chunk's 450).
 constexpr int kJoinRows = 32;
 
 template <int DP, bool BF16, bool MASK>
 __global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_rows_kernel(const Kv8AttnParams p, int G, int tile, int unit) {
     constexpr float U = MASK ? kLog2e : 1.f;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.c.D, groups = tile / kJoinRows;
+    constexpr int V = DP == 256 ? 2 : 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.c.D, rows = min(tile, kJoinRows), groups = tile / rows;
     const Plan pl(p, tile, unit);
-    const int eh = blockIdx.x / groups, qg = (blockIdx.x - eh * groups) * kJoinRows, e = eh / p.c.Hkv, h = eh - e * p.c.Hkv;
+    const int eh = blockIdx.x / groups, qg = (blockIdx.x - eh * groups) * rows, e = eh / p.c.Hkv, h = eh - e * p.c.Hkv;
     const Shares sh(p, pl, lane, e, h, G);
     pdl_wait_prerequisites();
     pdl_launch_dependents();
     if (sh.i0 == sh.i1) return;                                // one CTA had it all and wrote the outputs
-    const int last = static_cast<int>(min(static_cast<int64_t>(qg + kJoinRows), static_cast<int64_t>(sh.cnt) * pl.rep - sh.q0));
-    const int d = 4 * lane;
+    const int last = static_cast<int>(min(static_cast<int64_t>(qg + rows), static_cast<int64_t>(sh.cnt) * pl.rep - sh.q0));
 #pragma unroll 2
     for (int q = qg + warp; q < last; q += kJoinWarps) {
         float M = -INFINITY;
@@ -581,28 +582,38 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_rows_kernel(con
         for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
         const float ref = M == -INFINITY ? 0.f : M;
         float L = 0.f;
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 y[V];
+#pragma unroll
+        for (auto &v : y) v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
         for (int i = sh.i0; i <= sh.i1; ++i) {
             const int s = sh.slot(i);
             const float2 ml = slot_ml<DP>(p.ws, tile, G, s)[q];
             const float f = ex2((ml.x - ref) * U);
             L = fmaf(ml.y, f, L);
-            if (d < D) {
-                const float4 v = *reinterpret_cast<const float4 *>(slot_o<DP>(p.ws, tile, s) + static_cast<int64_t>(q) * DP + d);
-                y.x = fmaf(v.x, f, y.x);
-                y.y = fmaf(v.y, f, y.y);
-                y.z = fmaf(v.z, f, y.z);
-                y.w = fmaf(v.w, f, y.w);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const int d = 128 * k + 4 * lane;
+                if (d < D) {
+                    const float4 v = *reinterpret_cast<const float4 *>(slot_o<DP>(p.ws, tile, s) + static_cast<int64_t>(q) * DP + d);
+                    y[k].x = fmaf(v.x, f, y[k].x);
+                    y[k].y = fmaf(v.y, f, y[k].y);
+                    y[k].z = fmaf(v.z, f, y[k].z);
+                    y[k].w = fmaf(v.w, f, y[k].w);
+                }
             }
         }
         const int64_t qr = sh.q0 + q;
         const int tok = static_cast<int>(div64(qr, pl.rep)), hq = h * pl.rep + static_cast<int>(qr - static_cast<int64_t>(tok) * pl.rep);
         float so;
         const float f = out_factor<MASK>(M, L, p.sinks, hq, so) * so;
-        if (d < D)
-            store4<BF16>(p.out, (static_cast<int64_t>(sh.b) * p.r.T + tok) * p.ldo + static_cast<int64_t>(hq) * D + d,
-                         make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int d = 128 * k + 4 * lane;
+            if (d < D)
+                store4<BF16>(p.out, (static_cast<int64_t>(sh.b) * p.r.T + tok) * p.ldo + static_cast<int64_t>(hq) * D + d,
+                             make_float4(y[k].x * f, y[k].y * f, y[k].z * f, y[k].w * f));
+        }
     }
 }
 
@@ -620,29 +631,34 @@ int device_sms() {
 // Query tiles: 8 NT queries; larger ones share the decoded codes and are limited by registers (the queries'
 // digits take 3 DP / 16 * NT, the outputs DP / 4 * NT of them).
 int pick_nt(int DP, int64_t queries) {
-    const int most = DP == 64 ? 2 : DP == 128 ? 2 : 1;
-    const int want = queries <= 8 ? 1 : queries <= 16 ? 2 : 4;
-    return want < most ? want : most;
+    return queries <= 8 || DP == 256 ? 1 : 2;
 }
-// more queries a kv head than this go to 128-query tiles (kv8_tile.cu), where heads fit them
-constexpr int kTileFrom = 16;
+// More queries a kv head than this go to 128-query tiles (kv8_tile.cu), where heads fit them. us, tiles / this kernel,
+// at 40, 64, 96, 128 queries (bf16, D 128): 8 sequences of about 2250 rows 43 / 59, 45 / 70, 48 / 117, 51 / 146; one
+// sequence of 16000 rows 53 / 33, 55 / 38, 58 / 53, 62 / 66.
+constexpr int kTileFrom = 64;
 bool use_tiles(int D, int64_t queries) { return D <= 128 && queries > kTileFrom; }
 int padded_dim(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 // after a split kernel of G CTAs over units of `unit` rows and tiles of `tile` queries
-template <int DP, bool BF16, bool MASK, bool ROWS>
+template <int DP, bool BF16, bool MASK>
 cudaError_t join_launch(const Kv8AttnParams &p, int G, int tile, int unit, cudaStream_t s) {
     const int64_t tiles = (static_cast<int64_t>(p.r.T) * (p.Hq / p.c.Hkv) + tile - 1) / tile;
-    const int64_t joins = tiles * p.c.B * p.c.Hkv * (ROWS ? tile / kJoinRows : tile);
+    // with a quarter as many segments as CTAs or more a segment has about five parts at most; with fewer, a whole CTA adds
+    // one query's. One token of 64 sequences (256 segments): XXX us by rows, 58.1 by queries; one sequence of 131001 rows
+    // (8 segments, 55 parts each): XXX by rows, 49.5 by queries.
+    const int64_t segments = tiles * p.c.B * p.c.Hkv;
+    const bool by_rows = segments * 4 >= G;
+    const int64_t joins = segments * (by_rows ? tile / std::min(tile, kJoinRows) : tile);
     if (joins > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    return launch_pdl(ROWS ? kv8_attn_join_rows_kernel<DP, BF16, MASK> : kv8_attn_join_kernel<DP, BF16, MASK>,
+    return launch_pdl(by_rows ? kv8_attn_join_rows_kernel<DP, BF16, MASK> : kv8_attn_join_kernel<DP, BF16, MASK>,
                       dim3(static_cast<unsigned>(joins)), dim3(kJoinWarps * 32), 0, s, p, G, tile, unit);
 }
 
 template <int DP, int NT, bool BF16, bool MASK>
 struct Split {
     // rows a warp takes in a step, stages: 12 warps per SM (the registers' limit for small tiles) x 2 x 8 KB
-    static constexpr int R = DP == 256 || NT == 4 ? 1 : 2, NS = R == 1 ? 3 : 2;
+    static constexpr int R = DP == 256 ? 1 : 2, NS = R == 1 ? 3 : 2;
     static constexpr int ring = kWarps * NS * kStageBytes<DP, R>, merge = kMergeBytes<DP, NT>;
     static constexpr int smem = 1024 + (ring > merge ? ring : merge);
     static int ctas() {                                        // one resident wave
@@ -667,16 +683,13 @@ struct Split {
         const cudaError_t e = launch_pdl(kv8_attn_split_kernel<DP, NT, BF16, MASK, R, NS>, dim3(G), dim3(kWarps * 32), smem, s,
                                          mk, mv, p);
         if (e != cudaSuccess) return e;
-        return join_launch<DP, BF16, MASK, false>(p, G, 8 * NT, kWarps * 16 * R, s);
+        return join_launch<DP, BF16, MASK>(p, G, 8 * NT, kWarps * 16 * R, s);
     }
 };
 
 // f(Split<...>) for the call's sizes and types
 template <int DP, bool BF16, bool MASK, typename F>
 auto with_nt(int nt, F f) {
-    if constexpr (DP == 64) {
-        if (nt == 4) return f(Split<DP, 4, BF16, MASK>{});
-    }
     if constexpr (DP != 256) {
         if (nt == 2) return f(Split<DP, 2, BF16, MASK>{});
     }
@@ -723,8 +736,8 @@ cudaError_t kv8_attn_launch(const Kv8AttnParams &p, bool bf16, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const auto join = [&](auto dp) {
         constexpr int DP = decltype(dp)::value;
-        if (bf16) return p.mask ? join_launch<DP, true, true, true>(p, G, tile, unit, s) : join_launch<DP, true, false, true>(p, G, tile, unit, s);
-        return p.mask ? join_launch<DP, false, true, true>(p, G, tile, unit, s) : join_launch<DP, false, false, true>(p, G, tile, unit, s);
+        if (bf16) return p.mask ? join_launch<DP, true, true>(p, G, tile, unit, s) : join_launch<DP, true, false>(p, G, tile, unit, s);
+        return p.mask ? join_launch<DP, false, true>(p, G, tile, unit, s) : join_launch<DP, false, false>(p, G, tile, unit, s);
     };
     return p.c.D <= 64 ? join(std::integral_constant<int, 64>{}) : join(std::integral_constant<int, 128>{});
 }

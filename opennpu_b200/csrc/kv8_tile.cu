@@ -229,10 +229,6 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
                 const uint32_t stm = tmem + lanes + buf * kRows;
                 const float scj = sc;
                 if (j + 1 < n) sc = load_scale(r0 + kRows);
-                const uint32_t sphase = QT == 2 ? ns & 1 : ns >> 1 & 1;
-                if (!failed) failed = __any_sync(0xffffffffu, !mbar_wait_bounded(s_full + 8 * buf, sphase, kWaitNs));
-                ++ns;
-                tc_fence_after();
                 const bool live = edge > 0;                      // a warp without a valid query leaves its lanes of P as they are
                 // V's largest scale (bits: NaN does not count) against the weights' power of two
                 uint32_t vb = lane >= 8 && lane < 16 ? __float_as_uint(scj) : 0u;
@@ -258,10 +254,24 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
                     if (cv != 0.f) rescale_o(cn / cv);
                     cv = cn;
                 }
-                const float vv = cv * scj, lg = __log2f(vv), rv = 1.f / vv;
-                const auto scale_k = [&](int g) { return rs * __shfl_sync(0xffffffffu, scj, g); };
+                // what the four 16-column groups of this half need: K's scale with the query's, V's with the power of two
+                float fk[4], wv[4], lg[4], rv[4];
+                {
+                    const float vv = cv * scj, lv = __log2f(vv), iv = __frcp_rn(vv);
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        fk[g] = rs * __shfl_sync(0xffffffffu, scj, 4 * hf + g);
+                        wv[g] = __shfl_sync(0xffffffffu, vv, 8 + 4 * hf + g);
+                        lg[g] = __shfl_sync(0xffffffffu, lv, 8 + 4 * hf + g);
+                        rv[g] = __shfl_sync(0xffffffffu, iv, 8 + 4 * hf + g);
+                    }
+                }
                 const bool above0 = !(lane >= 8 && lane < 16 && !(scj > 0.f));
                 const bool usual = !MASK && r0 + kRows <= edge && __all_sync(0xffffffffu, above0);
+                const uint32_t sphase = QT == 2 ? ns & 1 : ns >> 1 & 1;
+                if (!failed) failed = __any_sync(0xffffffffu, !mbar_wait_bounded(s_full + 8 * buf, sphase, kWaitNs));
+                ++ns;
+                tc_fence_after();
                 // a finished score of the tile's column, -inf where it is not seen
                 const auto score = [&](uint32_t s, float f, int col) {
                     const float x = __uint_as_float(s) * f;
@@ -274,14 +284,14 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
                 // the largest score of this half
                 float top = -INFINITY;
                 if (live) {
-#pragma unroll 1
-                    for (int ch = 2 * hf; ch < 2 * hf + 2; ++ch) {
+#pragma unroll
+                    for (int ch = 0; ch < 2; ++ch) {
                         uint32_t s[32];
-                        tc_ld_issue_x32(stm + 32 * ch, s);
+                        tc_ld_issue_x32(stm + 64 * hf + 32 * ch, s);
                         tc_wait_ld32(s);
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
-                            const float f = scale_k(2 * ch + g);
+                            const float f = fk[2 * ch + g];
                             if (usual) {                         // scales are not negative
                                 float t0 = __uint_as_float(s[16 * g]), t1 = __uint_as_float(s[16 * g + 1]);
 #pragma unroll
@@ -293,7 +303,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
                                 top = fmaxf(top, fmaxf(t0, t1) * f);
                             } else {
 #pragma unroll
-                                for (int k = 0; k < 16; ++k) top = fmaxf(top, score(s[16 * g + k], f, r0 + 32 * ch + 16 * g + k));
+                                for (int k = 0; k < 16; ++k) top = fmaxf(top, score(s[16 * g + k], f, r0 + 64 * hf + 32 * ch + 16 * g + k));
                             }
                         }
                     }
@@ -313,7 +323,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
                 }
                 // the weights of this half
                 if (live) {
-#pragma unroll 1
+#pragma unroll
                     for (int ch = 0; ch < 2; ++ch) {
                         uint32_t s[32], ph[16], pw[16];
                         tc_ld_issue_x32(stm + 64 * hf + 32 * ch, s);
@@ -327,13 +337,12 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
                         };
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
-                            const int gi = 4 * hf + 2 * ch + g;
-                            const float f = scale_k(gi);
+                            const float f = fk[2 * ch + g];
                             float s0 = 0.f, s1 = 0.f;
                             if (usual) {
                                 // V's scales are above 0: a weight is one exponential, w = 2^(S f - m + log2(s_v c)), and the
                                 // sum takes w / (s_v c)
-                                const float at = __shfl_sync(0xffffffffu, lg, 8 + gi) - m;
+                                const float at = lg[2 * ch + g] - m;
 #pragma unroll
                                 for (int k = 0; k < 16; k += 2) {
                                     const float w0 = ex2(fmaf(__uint_as_float(s[16 * g + k]), f, at));
@@ -342,9 +351,9 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
                                     s1 += w1;
                                     keep(8 * g + k / 2, w0, w1);
                                 }
-                                l = fmaf(s0 + s1, __shfl_sync(0xffffffffu, rv, 8 + gi), l);
+                                l = fmaf(s0 + s1, rv[2 * ch + g], l);
                             } else {
-                                const float wv = __shfl_sync(0xffffffffu, vv, 8 + gi);
+                                const float wg = wv[2 * ch + g];
                                 const int col = r0 + 64 * hf + 32 * ch + 16 * g;
 #pragma unroll
                                 for (int k = 0; k < 16; k += 2) {
@@ -353,7 +362,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
                                     s0 += e0;
                                     s1 += e1;
                                     // a row that is not seen weighs nothing, even where its scale is NaN
-                                    keep(8 * g + k / 2, x0 == -INFINITY ? 0.f : e0 * wv, x1 == -INFINITY ? 0.f : e1 * wv);
+                                    keep(8 * g + k / 2, x0 == -INFINITY ? 0.f : e0 * wg, x1 == -INFINITY ? 0.f : e1 * wg);
                                 }
                                 l += s0 + s1;
                             }
