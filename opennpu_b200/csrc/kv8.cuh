@@ -68,10 +68,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {     // NaN where ei
 // An entry is a (sequence, query tile); its rows are counted in units of `unit` rows, once per kv head.
 struct Plan {
     int rep, tile, tiles, entries, unit;    // query heads per kv head, queries a tile, tiles a sequence, B * tiles
+    int shift;                              // unit = 1 << shift
     __device__ __forceinline__ Plan(const Kv8AttnParams &p, int tile_, int unit_) {
         rep = p.Hq / p.c.Hkv;
         tile = tile_;
         unit = unit_;
+        shift = 31 - __clz(unit);
         tiles = static_cast<int>((static_cast<int64_t>(p.r.T) * rep + tile - 1) / tile);
         entries = p.c.B * tiles;
     }
@@ -85,10 +87,12 @@ struct Plan {
         if (first >= cnt) return 0;
         return pos + min(last, cnt - 1) + 1;
     }
+    __device__ __forceinline__ int units_of(int len) const {
+        return static_cast<int>((static_cast<unsigned>(len) + unit - 1) >> shift);
+    }
     __device__ __forceinline__ int units(const Kv8AttnParams &p, int e) const {
         int pos, cnt;
-        const unsigned n = rows(p, e, pos, cnt);
-        return static_cast<int>((n + unit - 1) / unit);
+        return units_of(rows(p, e, pos, cnt));
     }
 };
 __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
@@ -151,30 +155,53 @@ __device__ __forceinline__ int64_t total_units(const Kv8AttnParams &p, const Pla
 // A CTA's way through the list: segments, each a run of one entry's units for one kv head
 struct Walk {
     int64_t u, u1, e0;                // the next unit, the end of this CTA's, the entry's first
-    int e, n;                         // the entry and its units (per head)
+    int e, n, pos, cnt, len;          // the entry, its units (per head), its sequence's rows, the rows it sees
     bool first;                       // no segment taken yet
     // the segment at u
-    int b, h, ua, ub, pos, cnt, len, nq;
+    int b, h, ua, ub, nq;
     int64_t q0;                       // the tile's first query
     __device__ __forceinline__ bool start(const Kv8AttnParams &p, const Plan &pl, int lane, int cta, int G) {
+        first = true;
+        if (pl.entries <= 32) {       // one round of loads: an entry a lane (their units fit 32 bits)
+            int ps = 0, cn = 0, ln = 0;
+            if (lane < pl.entries) ln = pl.rows(p, lane, ps, cn);
+            const unsigned mine = pl.units_of(ln);
+            unsigned incl = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned up = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += up;
+            }
+            const int64_t N = static_cast<int64_t>(__shfl_sync(0xffffffffu, incl, 31)) * p.c.Hkv, per = units_per_cta(N, G);
+            u = per * cta;
+            u1 = min(N, u + per);
+            if (u >= u1) return false;
+            e = __ffs(__ballot_sync(0xffffffffu, static_cast<int64_t>(incl) * p.c.Hkv > u)) - 1;
+            n = __shfl_sync(0xffffffffu, mine, e);
+            e0 = (static_cast<int64_t>(__shfl_sync(0xffffffffu, incl, e)) - n) * p.c.Hkv;
+            pos = __shfl_sync(0xffffffffu, ps, e);
+            cnt = __shfl_sync(0xffffffffu, cn, e);
+            len = __shfl_sync(0xffffffffu, ln, e);
+            return true;
+        }
         const int64_t N = total_units(p, pl, lane), per = units_per_cta(N, G);
         u = per * cta;
         u1 = min(N, u + per);
         if (u >= u1) return false;
         find_entry(p, pl, lane, u, e, n, e0);
-        first = true;
+        len = pl.rows(p, e, pos, cnt);
         return true;
     }
     __device__ __forceinline__ bool segment(const Kv8AttnParams &p, const Plan &pl) {
         if (u >= u1) return false;
         while (n == 0 || u >= e0 + static_cast<int64_t>(n) * p.c.Hkv) {     // the next entry with rows
             e0 += static_cast<int64_t>(n) * p.c.Hkv;
-            n = pl.units(p, ++e);
+            len = pl.rows(p, ++e, pos, cnt);
+            n = pl.units_of(len);
         }
         h = static_cast<int>(div64(u - e0, n));
         ua = static_cast<int>(u - e0 - static_cast<int64_t>(h) * n);
         ub = static_cast<int>(min(static_cast<int64_t>(n), ua + (u1 - u)));
-        len = pl.rows(p, e, pos, cnt);
         b = pl.tiles == 1 ? e : e / pl.tiles;
         q0 = static_cast<int64_t>(e - b * pl.tiles) * pl.tile;
         nq = static_cast<int>(min(static_cast<int64_t>(pl.tile), static_cast<int64_t>(cnt) * pl.rep - q0));
@@ -202,8 +229,7 @@ struct Shares {
             if (i < e) before += v;
         }
         int pos;
-        const unsigned len = pl.rows(p, e, pos, cnt);
-        const int n = static_cast<int>((len + pl.unit - 1) / pl.unit);
+        const int n = pl.units_of(pl.rows(p, e, pos, cnt));
         b = pl.tiles == 1 ? e : e / pl.tiles;
         q0 = static_cast<int64_t>(e - b * pl.tiles) * pl.tile;
         const int64_t N = warp_sum64(all) * p.c.Hkv, u = warp_sum64(before) * p.c.Hkv + static_cast<int64_t>(h) * n;

@@ -105,6 +105,10 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __gri
 #pragma unroll
         for (int s = 0; s < NS; ++s) mbar_init(bar0 + 8 * s, 1);
         mbar_init_fence();
+        if (warp == 0) {                  // the maps are launch parameters: their fetch need not wait
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&mapk) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&mapv) : "memory");
+        }
     }
     const uint64_t pol = l2_evict_first_policy();
     __syncwarp();
