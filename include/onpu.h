@@ -398,7 +398,7 @@ int onpu_attn_step_dev(const float *q, int Hq, int D, const void *K, const void 
 typedef struct onpu_kv8_cache {
     int8_t *k, *v;           /* codes of row j, head h, sequence b at b * bs + h * hs + j * rs, dim of them; */
                              /* 16-byte aligned, strides multiples of 16, rs >= dim                          */
-    float *k_scale, *v_scale;/* scale of row j at b * sbs + h * shs + j / block                               */
+    float *k_scale, *v_scale;/* scale of row j at b * sbs + h * shs + j / block; not negative                  */
     int64_t batch, heads, rows, dim;  /* sequences, kv heads, rows a sequence can hold, head size           */
     int64_t bs, hs, rs;      /* strides of k and v in codes                                                  */
     int64_t sbs, shs;        /* strides of the scales in floats                                              */
@@ -412,7 +412,7 @@ typedef struct onpu_kv8_cache {
  * multiple of 16 bytes. dim is a multiple of 16, at most 256; batch at most 32767. A sequence whose rows are
  * not all inside the cache, or whose cnt is not in [0, T], is skipped and sets the device status
  * (onpu_check_device). Asynchronous on `stream`, no allocation, capturable; calls that touch the same
- * sequence's rows are ordered by the caller. The device that is current must be the library's.
+ * sequence's rows are ordered by the caller, and pos and cnt stay as they are until a call is done. The device that is current must be the library's.
  * 0 ok, < 0 error.
  *
  * append: quantises rows k, v [batch * T][heads * dim] into the cache. For each block that holds one

@@ -52,11 +52,11 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 __device__ __forceinline__ float2 unpack_h2(uint32_t x) { return __half22float2(*reinterpret_cast<__half2 *>(&x)); }
-// 2^(top - exponent of x), its exponent kept within +-100: x times it is in [2^top, 2^(top + 1)); 1 for 0, inf and NaN
+// 2^(top - exponent of x), at most 2^126: x times it is in [2^top, 2^(top + 1)) (less for x below 2^(top - 126)); 1 for 0, inf and NaN
 __device__ __forceinline__ float pow2_to(float x, int top) {
     const int e = static_cast<int>(__float_as_uint(x) >> 23 & 0xff);
     if (e == 255 || !(fabsf(x) > 0.f)) return 1.f;
-    return __uint_as_float(static_cast<uint32_t>(127 + min(100, max(-100, top + 127 - e))) << 23);
+    return __uint_as_float(static_cast<uint32_t>(127 + min(126, max(-126, top + 127 - e))) << 23);
 }
 __device__ __forceinline__ float max_nan(float a, float b) {     // NaN where either is
     float d;
@@ -144,6 +144,11 @@ __device__ __forceinline__ void find_entry(const Kv8AttnParams &p, const Plan &p
             return;
         }
         e0 += __shfl_sync(0xffffffffu, incl, 31);
+        if (base + 32 >= pl.entries) {           // only if pos or cnt changed under the call: nothing for this CTA
+            e = pl.entries - 1;
+            n = 0;
+            return;
+        }
     }
 }
 // units of all entries and heads
@@ -196,7 +201,8 @@ struct Walk {
         if (u >= u1) return false;
         while (n == 0 || u >= e0 + static_cast<int64_t>(n) * p.c.Hkv) {     // the next entry with rows
             e0 += static_cast<int64_t>(n) * p.c.Hkv;
-            len = pl.rows(p, ++e, pos, cnt);
+            if (++e >= pl.entries) return false;     // only if pos or cnt changed under the call
+            len = pl.rows(p, e, pos, cnt);
             n = pl.units_of(len);
         }
         h = static_cast<int>(div64(u - e0, n));

@@ -19,6 +19,7 @@
 #include <mutex>
 #include <set>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "gpu_layout.cuh"
@@ -2722,6 +2723,19 @@ int onpu_attn_step_dev(const float *q, int Hq, int D, const void *K, const void 
 
 // ------------------------------------------------------------------ 8-bit KV cache
 namespace {
+// whether rows of n elements (count s0 apart, heads s1, sequences s2) share elements: each dimension, by growing
+// stride, has to step over all of the ones before
+bool kv8_overlap(int64_t n, int64_t c0, int64_t s0, int64_t s1, int64_t c1, int64_t s2, int64_t c2) {
+    std::pair<int64_t, int64_t> d[3] = {{s0, c0}, {s1, c1}, {s2, c2}};
+    std::sort(d, d + 3);
+    int64_t extent = n;
+    for (const auto &[stride, count] : d) {
+        if (count <= 1) continue;
+        if (stride < extent) return true;
+        extent = stride * (count - 1) + extent;
+    }
+    return false;
+}
 // What every kv8 call checks first: the cache's description and the token count. Fills c and r.
 bool kv8_check(const char *who, const onpu_kv8_cache *d, int64_t T, const int32_t *pos, const int32_t *cnt,
                Kv8Cache &c, Kv8Rows &r) {
@@ -2729,9 +2743,9 @@ bool kv8_check(const char *who, const onpu_kv8_cache *d, int64_t T, const int32_
         set_err("%s: a null cache, codes, scales or pos pointer", who);
         return false;
     }
-    if (d->batch < 1 || d->batch > 32767 || d->heads < 1 || d->heads > 65535 || d->rows < 1 || d->rows > 0x7fffffc0 ||
+    if (d->batch < 1 || d->batch > 32767 || d->heads < 1 || d->heads > 65535 || d->rows < 1 || d->rows > 0x7fffff00 ||
         d->dim < 16 || d->dim > 256 || d->dim % 16 || (d->block != 16 && d->block != 32 && d->block != 64)) {
-        set_err("%s: need 1 <= batch <= 32767, 1 <= heads <= 65535, 1 <= rows < 2^31 - 64, dim a multiple of 16 up to "
+        set_err("%s: need 1 <= batch <= 32767, 1 <= heads <= 65535, 1 <= rows <= 2^31 - 256, dim a multiple of 16 up to "
                 "256, block 16, 32 or 64 (got %lld, %lld, %lld, %lld, %d)", who, static_cast<long long>(d->batch),
                 static_cast<long long>(d->heads), static_cast<long long>(d->rows), static_cast<long long>(d->dim),
                 d->block);
@@ -2745,8 +2759,12 @@ bool kv8_check(const char *who, const onpu_kv8_cache *d, int64_t T, const int32_
         return false;
     }
     const int64_t nb = (d->rows + d->block - 1) / d->block;
-    if ((d->heads > 1 && d->shs < nb) || (d->batch > 1 && d->sbs < nb)) {
-        set_err("%s: the scales need strides of at least rows / block", who);
+    if ((d->heads > 1 && d->shs < nb) || (d->batch > 1 && d->sbs < nb) || kv8_overlap(1, nb, 1, d->shs, d->heads, d->sbs, d->batch)) {
+        set_err("%s: the scales need strides of at least rows / block, no two of them in one place", who);
+        return false;
+    }
+    if (kv8_overlap(d->dim, d->rows, d->rs, d->hs, d->heads, d->bs, d->batch)) {
+        set_err("%s: the strides put codes of two rows in one place", who);
         return false;
     }
     if (T < 0 || T > 0x7fffffff) {
@@ -2799,6 +2817,10 @@ int onpu_kv8_append_dev(const onpu_kv8_cache *cache, const void *k, int64_t ldk,
     Kv8Cache c;
     Kv8Rows r;
     if (!kv8_check(who, cache, T, pos, cnt, c, r)) return -1;
+    if (c.k == c.v || c.ks == c.vs) {
+        set_err("%s: K and V are the same codes or scales", who);
+        return -1;
+    }
     if (T == 0) return 0;
     const int64_t n = cache->heads * cache->dim, rows = cache->batch * T;
     if (!kv8_check_rows(who, "k", k, ldk, n, rows, x_bf16) || !kv8_check_rows(who, "v", v, ldv, n, rows, x_bf16) ||

@@ -30,7 +30,8 @@ def call(fn, d, rows=1 << 24, ld=256, T=3, bf16=1, pos=1 << 25, Hq=8, ws=1 << 26
 BAD_CACHE = [dict(k=0), dict(v_scale=0), dict(batch=0), dict(batch=32768), dict(heads=0), dict(rows=0),
              dict(rows=1 << 31), dict(dim=72), dict(dim=272), dict(dim=0), dict(block=8), dict(block=48),
              dict(k=(1 << 20) + 8), dict(v=(1 << 21) + 1), dict(k_scale=(1 << 22) + 2), dict(bs=4 * 100 * 64 + 8),
-             dict(hs=8), dict(hs=0), dict(bs=0), dict(bs=-1024), dict(rs=48), dict(rs=72), dict(shs=3), dict(sbs=0)]
+             dict(hs=8), dict(hs=0), dict(bs=0), dict(bs=-1024), dict(rs=48), dict(rs=72), dict(shs=3), dict(sbs=0),
+             dict(rows=(1 << 31) - 255), dict(hs=64, bs=400 * 64), dict(bs=2 * 100 * 64), dict(sbs=8), dict(shs=4, sbs=4)]
 
 
 @pytest.mark.parametrize("fn", ["append", "read", "attn"])
@@ -60,6 +61,11 @@ BAD_CALL = [("append", dict(rows=(1 << 24) + 8), "k"), ("append", dict(ld=255), 
 def test_bad_rows_heads_and_workspace_are_refused(fn, bad, what):
     assert call(fn, desc(), **bad) < 0
     assert what in L.last_error() and "onpu_kv8_" + fn in L.last_error()
+
+
+def test_append_refuses_one_buffer_for_both():
+    assert call("append", desc(v=GOOD["k"])) < 0 and "same" in L.last_error()
+    assert call("append", desc(v_scale=GOOD["k_scale"])) < 0 and "same" in L.last_error()
 
 
 def test_no_tokens_is_no_call():

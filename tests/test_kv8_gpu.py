@@ -289,6 +289,60 @@ def test_what_masked_rows_hold_does_not_matter(T, dtype):
     assert torch.isfinite(y[1]).all() and torch.isfinite(y[0, 1:]).all()
 
 
+@pytest.mark.parametrize("T,dtype", [(1, "fp32"), (1, "bf16"), (3, "fp32"), (64, "bf16"), (40, "fp32")])
+@pytest.mark.parametrize("power", [121, -100])
+def test_queries_and_scales_at_the_ends_of_the_range(T, dtype, power):
+    """Queries times 2^power over keys times 2^-power give the scores they give at 1; values near 2^100 and
+    2^-100; a head of zero queries weighs rows equally; a query that is not finite gives NaN, alone."""
+    B, Hq, H, D, S, block = 2, 6, 2, 64, 150, 32
+    rng = np.random.default_rng(T)
+    cache = rand_cache(rng, B, H, S, D, block)
+    cache[2][:] = cache[2] * np.float32(2.0 ** -power)
+    cache[3][:] = cache[3] * np.float32(2.0 ** (100 if power > 0 else -100))
+    q, qt = rand_rows(rng, (B, T, Hq, D), dtype)
+    q, qt = q * np.float32(2.0 ** power), qt * 2.0 ** power
+    q[:, :, 2], qt[:, :, 2] = 0, 0
+    c = bind(cache, block)
+    pos, cnt = [S - T, 20], [T, T]
+    y = c.attn(qt, i32(pos))
+    check_attn(y, q, cache, block, pos, cnt, bf16=dtype == "bf16")
+    qt[0, T - 1, 1, 5] = float("inf")
+    qt[1, 0, 4, 0] = float("nan")
+    z = c.attn(qt, i32(pos))
+    same = torch.ones(B, T, Hq, dtype=torch.bool)
+    same[0, T - 1, 1] = same[1, 0, 4] = False
+    assert torch.equal(z[same], y[same]) and torch.isnan(z[~same]).all()
+
+
+def test_negative_and_zero_scale():
+    B, Hq, H, D, S = 1, 4, 2, 64, 200
+    rng = np.random.default_rng(2)
+    cache = rand_cache(rng, B, H, S, D, 32)
+    c = bind(cache, 32)
+    for T, dtype in ((1, "fp32"), (1, "bf16"), (80, "bf16")):
+        q, qt = rand_rows(rng, (B, T, Hq, D), dtype)
+        for scale in (-0.3, 0.0):
+            y = c.attn(qt, i32([S - T]), scale=scale)
+            check_attn(y, q, cache, 32, [S - T], [T], scale=scale, bf16=dtype == "bf16")
+
+
+def test_scores_that_grow_along_the_rows():
+    """Later rows outweigh all earlier ones again and again: the reference moves in every step, by a little
+    and by more than fp16 spans; and a value scale that grows past the weights' range."""
+    B, Hq, H, D, S, block = 1, 8, 2, 128, 1500, 16
+    rng = np.random.default_rng(4)
+    cache = list(rand_cache(rng, B, H, S, D, block))
+    for steep in (0.02, 0.6):
+        cache[0][...] = 100
+        cache[2][...] = (steep * np.arange(cache[2].shape[2]) / (100 * D) * D ** 0.5).astype(np.float32)
+        cache[3][...] = (2.0 ** (np.arange(cache[3].shape[2]) // 4 - 12)).astype(np.float32)
+        c = bind(tuple(cache), block)
+        for T, dtype in ((1, "fp32"), (1, "bf16"), (60, "bf16"), (40, "fp32")):
+            q = np.ones((B, T, Hq, D), np.float32)
+            y = c.attn(torch.from_numpy(q).to(DT[dtype]).cuda(), i32([S - T]))
+            check_attn(y, q, cache, block, [S - T], [T], bf16=dtype == "bf16")
+
+
 def test_strides_slices_and_broadcast_masks():
     """A cache kept [B, rows, heads, dim], sequences sliced out of a larger cache, q / k / v as slices of
     fused projection rows, masks broadcast over sequences and tokens, a scale and an out of the caller's."""
