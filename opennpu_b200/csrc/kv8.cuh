@@ -105,12 +105,9 @@ __device__ __forceinline__ int64_t div64(int64_t a, int64_t b) {
     if (((a | b) >> 31) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
     return a / b;
 }
-// units a CTA takes: N units over G CTAs, at least kMinUnits each (a part shorter than that costs more to
-// join than it saves); CTA i has units [i * per, (i + 1) * per) of the list
-constexpr int kMinUnits = 1;
-__device__ __forceinline__ int64_t units_per_cta(int64_t N, int G) {
-    return max(static_cast<int64_t>(kMinUnits), div64(N + G - 1, G));
-}
+// units a CTA takes: N units over G CTAs; CTA i has units [i * per, (i + 1) * per) of the list. (At least two each: one
+// token over 4096 rows 10.0 us against 10.5, over 77 rows 9.5 against 6.3.)
+__device__ __forceinline__ int64_t units_per_cta(int64_t N, int G) { return max(int64_t{1}, div64(N + G - 1, G)); }
 
 // ws: per CTA two slots of [tile][DP] outputs, then per slot [tile] (reference, sum) pairs
 template <int DP>

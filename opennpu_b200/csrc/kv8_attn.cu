@@ -4,26 +4,31 @@
 // with an online softmax in fp32; a query whose mask leaves no row gives zeros.
 //
 // The T * Hq / Hkv queries that share a kv head are the columns of the products (8 NT of them a tile), so
-// each cache row is read once for all of a tile: a warp takes 16 rows a step,
-//   X[row][query] = K[row][:] . q[query][:]       mma m16n8k16, A = 16 rows of K
-//   O^T[d][query] += V^T[d][row] . P^T[row][query]   A = V^T
-// The codes become fp16 exactly (|c| <= 127). Which k of the product is which d is free, so a lane reads 16
-// bytes of its rows from shared memory and uses them as they lie; for V a lane reads the same bytes of
-// four rows and pairs them with byte permutes, so nothing is transposed. K's scale multiplies the finished
-// scores, V's the weights.
-//  * q is scaled by a power of two to [256, 512) and rounded to fp16: exact for bf16 but for values 2^-22
-//    below the row's largest, and two fp16 parts (22 bits) for fp32 calls.
-//  * weights: w = 2^(x - m) * s_v * c, c a power of two that keeps s_v * c in [2^7, 2^9], rounded to fp16 (one
-//    part for bf16 outputs: 2^-11 of a weight against the output's 2^-8; two parts, 22 bits, for fp32).
+// each cache row is read once for all of a tile: a warp takes 16 R rows a step,
+//   X[row][query] = K[row][:] . q[query][:]          m16n8k32 int8, A = 16 rows of K
+//   O^T[d][query] += V^T[d][row] . P^T[row][query]   m16n8k16 fp16, A = V^T
+// Which k of a product is which d or row is free, so a lane reads 16 bytes of its rows from shared memory and uses
+// them as they lie; for V a lane reads the same bytes of four rows and pairs them with byte permutes, so nothing
+// is transposed. K's scale multiplies the finished scores, V's the weights.
+//  * q is taken as three base-256 digits of q f, f a power of two that puts the row's largest |q f| in [2^22, 2^23): 24
+//    bits of the row's largest value, and sums of codes times digits that are exact. K's codes need no
+//    decoding, and an int8 product has twice the k of an fp16 one at the same rate (4.4 ns a warp
+//    instruction on one of an SM's four quarters, both). Against fp16 q (two parts for fp32) and decoded K, with cp.async:
+//    one token over 131001 rows 65.0 -> 49.5 us, 484 warp instructions per 16 rows before.
+//  * weights: w = 2^(x - m) * s_v * c, c a power of two that keeps s_v * c below 2^9, rounded to fp16 (one
+//    part for bf16 outputs: 2^-11 of a weight against the output's 2^-8; two parts, 22 bits, for fp32), times V's codes
+//    as fp16, exactly (|c| <= 127): 0x64uu is 1024 + uu.
 //  * m is a reference within 2^6 (no mask) or e^4 (mask) of the running maximum, raised only when a score
 //    passes it by more: the accumulators are rescaled a few times a sequence, not every step. With a mask
 //    scores stay in natural units, x - m is formed first, so masks of the lowest finite value stay finite.
 //
-// Bound by HBM on the cache (2 D + 8 / block bytes a row and head) while a tile has few queries. The rows
-// of all sequences, tiles and heads are one list of 64-row units (from pos and cnt, on the device), cut
-// evenly over one wave of CTAs whatever the lengths are; a CTA writes finished outputs for the
-// (sequence, tile, head) it covers alone and a partial (reference, sum, output) for at most two it shares, which a second launch
-// adds in CTA order.
+// Bound by HBM on the cache (2 D + 8 / block bytes a row and head) while a tile has few queries: 5.3 TB/s at 131001
+// rows (0.82 of the copy bandwidth), 4.5 TB/s for 64 sequences of 100 to 8192 rows. Short calls are bound by the chain
+// of one step (place in the list, TMA and queries, products, softmax, merge: 3 to 4 us) and of the join (2 us).
+// The rows of all sequences, tiles and heads are one list of units of 64 R rows (from pos and cnt, on the device), cut
+// evenly over one wave of CTAs whatever the lengths are; a CTA writes finished outputs for the (sequence, tile, head)
+// it covers alone and a partial (reference, sum, output) for at most two it shares, which a second launch adds in CTA
+// order. That one is launched while the first runs and waits only with its place in the list found.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -207,7 +212,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __gri
                 uint32_t dg[3] = {0, 0, 0};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int Q = __float2int_rn(x[s][k] * f);
+                    const int Q = min(__float2int_rn(x[s][k] * f), 0x7fffff);     // 2^23 - 1/2 rounds up to 2^23
 #pragma unroll
                     for (int j = 0; j < 3; ++j) dg[j] |= static_cast<uint32_t>(Q >> (16 - 8 * j) & 0xff) << (8 * k);
                 }
@@ -649,8 +654,8 @@ template <int DP, bool BF16, bool MASK>
 cudaError_t join_launch(const Kv8AttnParams &p, int G, int tile, int unit, cudaStream_t s) {
     const int64_t tiles = (static_cast<int64_t>(p.r.T) * (p.Hq / p.c.Hkv) + tile - 1) / tile;
     // with a quarter as many segments as CTAs or more a segment has about five parts at most; with fewer, a whole CTA adds
-    // one query's. One token of 64 sequences (256 segments): XXX us by rows, 58.1 by queries; one sequence of 131001 rows
-    // (8 segments, 55 parts each): XXX by rows, 49.5 by queries.
+    // one query's. One token of 64 sequences (256 segments): 51.9 us by rows, 58.1 by queries; one sequence of 131001 rows
+    // (8 segments, 55 parts each): 56.8 by rows, 49.4 by queries.
     const int64_t segments = tiles * p.c.B * p.c.Hkv;
     const bool by_rows = segments * 4 >= G;
     const int64_t joins = segments * (by_rows ? tile / std::min(tile, kJoinRows) : tile);

@@ -18,6 +18,13 @@
 //  * one warp issues the products and owns tensor memory.
 // QT = 2 query tiles share a decoded row tile and alternate: one's softmax runs beside the other's products. QT = 1
 // (at most 128 queries, or fp32) alternates two S buffers instead.
+//
+// Measured: 512 tokens over 16.8k rows, 40 query heads on 8 kv heads of 128: 254 us (0.41 of the products' floor at the
+// measured bf16 rate; 1088 us in the kernel for few queries). With the work of a role left out, the same call takes 118 us
+// without any, 185 with the products alone, 209 with the decoding too: what is left besides the products is the chain from
+// one role to the next, several times per 128 rows, and the softmax's part of it. 128 columns a softmax thread: 280 to 298;
+// all 128 scores in registers: 382 (the unrolled code misses the instruction cache).
+//
 // Every wait is bounded (2 s) and reports through the error word.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

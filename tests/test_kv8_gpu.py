@@ -314,6 +314,20 @@ def test_queries_and_scales_at_the_ends_of_the_range(T, dtype, power):
     assert torch.equal(z[same], y[same]) and torch.isnan(z[~same]).all()
 
 
+@pytest.mark.parametrize("T,dtype", [(1, "fp32"), (1, "bf16"), (3, "fp32"), (70, "fp32"), (70, "bf16")])
+def test_queries_whose_largest_value_is_all_ones(T, dtype):
+    """The largest significand (2 - 2^-23, bf16 2 - 2^-7) of either sign: its rounded digits must not wrap."""
+    rng = np.random.default_rng(T)
+    cache = rand_cache(rng, 1, 2, 150, 64, 32)
+    c = bind(cache, 32)
+    q, _ = rand_rows(rng, (1, T, 4, 64), dtype)
+    top = np.float32(2 - (2.0 ** -23 if dtype == "fp32" else 2.0 ** -7)) * 4
+    q = np.clip(q, -7, 7)
+    q[..., 3], q[..., 40] = top, -top
+    y = c.attn(torch.from_numpy(q).to(DT[dtype]).cuda(), i32([150 - T]))
+    check_attn(y, q, cache, 32, [150 - T], [T], bf16=dtype == "bf16")
+
+
 def test_negative_and_zero_scale():
     B, Hq, H, D, S = 1, 4, 2, 64, 200
     rng = np.random.default_rng(2)
