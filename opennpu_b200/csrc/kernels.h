@@ -276,10 +276,10 @@ struct Kv8AttnParams {
 };
 int64_t kv8_attn_ws_bytes(int Hq, int Hkv, int D, int T, bool bf16);
 cudaError_t kv8_attn_launch(const Kv8AttnParams &p, bool bf16, cudaStream_t stream);
-// its kernel for many queries a kv head, D <= 128 (kv8_tile.cu): query tile, rows of a unit and CTAs of its list
-int kv8_tile_queries(int64_t queries, bool bf16);
+// its kernel for many bf16 queries a kv head, D <= 128 (kv8_tile.cu): query tile, rows of a unit and CTAs of its list
+int kv8_tile_queries(int64_t queries);
 int kv8_tile_rows();
 int kv8_tile_ctas();
-cudaError_t kv8_tile_launch(const Kv8AttnParams &p, bool bf16, cudaStream_t stream);
+cudaError_t kv8_tile_launch(const Kv8AttnParams &p, cudaStream_t stream);
 
 }  // namespace onpu_b200

@@ -413,12 +413,24 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __gri
                             const uint32_t r01 = prmt(y[0], y[1], hf ? 0x7362u : 0x5140u);
                             const uint32_t r23 = prmt(y[2], y[3], hf ? 0x7362u : 0x5140u);
                             const uint32_t a0 = h2_lo(r01), a1 = h2_hi(r01), a2 = h2_lo(r23), a3 = h2_hi(r23);
-#pragma unroll
-                            for (int pt = 0; pt < PARTS; ++pt)
+                            if constexpr (PARTS == 1) {
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt)
-                                    mma_f16(o[(v * 4 + w) * 2 + hf][nt], a0, a1, a2, a3, pb[i][pt][nt][0],
-                                            pb[i][pt][nt][1]);
+                                    mma_f16(o[(v * 4 + w) * 2 + hf][nt], a0, a1, a2, a3, pb[i][0][nt][0], pb[i][0][nt][1]);
+                            } else {
+                                // the tensor core cuts its sums off (towards 0), which adds up over a long run of rows: the
+                                // two products of 16 rows on their own, added in fp32 (64 sequences of 16k rows: 4.2e-6 of
+                                // the result's norm off without, 3.5e-7 with)
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                                    for (int pt = PARTS - 1; pt >= 0; --pt)
+                                        mma_f16(t, a0, a1, a2, a3, pb[i][pt][nt][0], pb[i][pt][nt][1]);
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) o[(v * 4 + w) * 2 + hf][nt][k] += t[k];
+                                }
+                            }
                         }
                     }
                 }
@@ -642,11 +654,12 @@ int device_sms() {
 int pick_nt(int DP, int64_t queries) {
     return queries <= 8 || DP == 256 ? 1 : 2;
 }
-// More queries a kv head than this go to 128-query tiles (kv8_tile.cu), where heads fit them. us, tiles / this kernel,
+// More queries a kv head than this go to 128-query tiles (kv8_tile.cu), where heads fit them and they are bf16 (the tiles'
+// sums over rows stay in the tensor core, which cuts them off: 7.4e-6 off after 16k rows, too much for fp32). us, tiles / this kernel,
 // at 40, 64, 96, 128 queries (bf16, D 128): 8 sequences of about 2250 rows 43 / 59, 45 / 70, 48 / 117, 51 / 146; one
 // sequence of 16000 rows 53 / 33, 55 / 38, 58 / 53, 62 / 66.
 constexpr int kTileFrom = 64;
-bool use_tiles(int D, int64_t queries) { return D <= 128 && queries > kTileFrom; }
+bool use_tiles(int D, int64_t queries, bool bf16) { return bf16 && D <= 128 && queries > kTileFrom; }
 int padded_dim(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 // after a split kernel of G CTAs over units of `unit` rows and tiles of `tile` queries
@@ -723,9 +736,9 @@ int64_t kv8_attn_ws_bytes(int Hq, int Hkv, int D, int T, bool bf16) {
     const int64_t queries = static_cast<int64_t>(T) * (Hq / Hkv);
     const int DP = padded_dim(D);
     int64_t G = 0, tile = 8 * pick_nt(DP, queries);
-    if (use_tiles(D, queries)) {
+    if (use_tiles(D, queries, bf16)) {
         G = kv8_tile_ctas();
-        tile = kv8_tile_queries(queries, bf16);
+        tile = kv8_tile_queries(queries);
     } else {
         for (const bool mask : {false, true}) {
             const int64_t g = with_split(D, queries, bf16, mask, [](auto k) { return static_cast<int64_t>(k.ctas()); });
@@ -737,16 +750,15 @@ int64_t kv8_attn_ws_bytes(int Hq, int Hkv, int D, int T, bool bf16) {
 
 cudaError_t kv8_attn_launch(const Kv8AttnParams &p, bool bf16, cudaStream_t s) {
     const int64_t queries = static_cast<int64_t>(p.r.T) * (p.Hq / p.c.Hkv);
-    if (!use_tiles(p.c.D, queries))
+    if (!use_tiles(p.c.D, queries, bf16))
         return with_split(p.c.D, queries, bf16, p.mask != nullptr, [&](auto k) { return k.launch(p, s); });
-    const int G = kv8_tile_ctas(), tile = kv8_tile_queries(queries, bf16), unit = kv8_tile_rows();
+    const int G = kv8_tile_ctas(), tile = kv8_tile_queries(queries), unit = kv8_tile_rows();
     if ((queries + tile - 1) / tile * p.c.B > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    const cudaError_t e = kv8_tile_launch(p, bf16, s);
+    const cudaError_t e = kv8_tile_launch(p, s);
     if (e != cudaSuccess) return e;
     const auto join = [&](auto dp) {
         constexpr int DP = decltype(dp)::value;
-        if (bf16) return p.mask ? join_launch<DP, true, true>(p, G, tile, unit, s) : join_launch<DP, true, false>(p, G, tile, unit, s);
-        return p.mask ? join_launch<DP, false, true>(p, G, tile, unit, s) : join_launch<DP, false, false>(p, G, tile, unit, s);
+        return p.mask ? join_launch<DP, true, true>(p, G, tile, unit, s) : join_launch<DP, true, false>(p, G, tile, unit, s);
     };
     return p.c.D <= 64 ? join(std::integral_constant<int, 64>{}) : join(std::integral_constant<int, 128>{});
 }

@@ -1,12 +1,12 @@
-// Attention over the 8-bit KV cache for many queries a kv head (prompt chunks, drafts): the formulas of kv8_attn.cu on
+// Attention over the 8-bit KV cache for many bf16 queries a kv head (prompt chunks): the formulas of kv8_attn.cu on
 // the 5th-generation tensor cores. What bounds it is the tensor pipe (4 D flops a query and row), so tiles are
 // 128 queries x 128 rows:
 //   S = Q . K^T      tcgen05 kind::f16, Q and the decoded codes of K from shared memory, S in tensor memory
 //   O += P . V       P (fp16, written over S) from tensor memory, the decoded codes of V from shared memory
 // The codes become fp16 exactly (|c| <= 127); K's scales multiply the finished scores, V's the weights, as in the
-// kernel for few queries, and so do its choices: q as fp16 scaled by a power of two to [256, 512) (bf16: exact but
-// for values 2^-22 below the row's largest; fp32: two parts, 22 bits), weights w = 2^(x - m) s_v c as fp16 (fp32
-// calls: two parts), m raised only when a score passes it by 2^6 (e^4 with a mask, scores then in natural units).
+// kernel for few queries, and so its choices: weights w = 2^(x - m) s_v c as fp16, m raised
+// only when a score passes it by 2^6 (e^4 with a mask, scores then in natural units). q is fp16 scaled by a power of two
+// to [256, 512): exact but for values 2^-22 below the row's largest.
 //
 // One CTA per SM walks its part of the list of units (128 rows of one tile and kv head; Walk). Warp roles:
 //  * softmax warps, eight per query tile: a thread is a query and one half of a row tile's columns, so that the time
@@ -17,7 +17,7 @@
 //    128-byte-swizzled layout, two stages each. K is read K-major, V (rows are K of the product) MN-major.
 //  * one warp issues the products and owns tensor memory.
 // QT = 2 query tiles share a decoded row tile and alternate: one's softmax runs beside the other's products. QT = 1
-// (at most 128 queries, or fp32) alternates two S buffers instead.
+// (at most 128 queries) alternates two S buffers instead.
 //
 // Measured: 512 tokens over 16.8k rows, 40 query heads on 8 kv heads of 128: 254 us (0.41 of the products' floor at the
 // measured bf16 rate; 1088 us in the kernel for few queries). With the work of a role left out, the same call takes 118 us
@@ -46,12 +46,12 @@ constexpr int kSub = kRows * 128;                        // bytes of 128 rows x 
 constexpr int kBars = 24;
 constexpr int kDec = 3;                                  // decode warps: 12 or 20 warps in all, 3 or 5 a scheduler
 
-template <int DP, int QT, int PARTS>
+template <int DP, int QT>
 struct TileSizes {
     static constexpr int tile = kRows * DP * 2;          // 128 rows of DP fp16: DP / 64 sub-tiles of 64
     static constexpr int raw = kRows * DP;               // 128 rows of codes
     static constexpr int share = QT * 2 * kRows * 4;     // a float per softmax thread
-    static constexpr int smem = (QT * PARTS + 4) * tile + 2 * raw + share + kBars * 8 + 16;
+    static constexpr int smem = (QT + 4) * tile + 2 * raw + share + kBars * 8 + 16;
     static_assert(smem <= 227 * 1024, "a CTA's shared memory");
     static constexpr int soft = 8 * QT, threads = (soft + kDec + 1) * 32;
 };
@@ -91,17 +91,17 @@ __device__ __forceinline__ void tma_codes(uint32_t dst, const CUtensorMap *map, 
         : "memory");
 }
 
-template <int DP, int QT, int PARTS, bool BF16, bool MASK>
-__global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
+template <int DP, int QT, bool MASK>
+__global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
     kv8_attn_tile_kernel(const __grid_constant__ CUtensorMap mapk, const __grid_constant__ CUtensorMap mapv,
                          const Kv8AttnParams p) {
-    using Z = TileSizes<DP, QT, PARTS>;
+    using Z = TileSizes<DP, QT>;
     constexpr int CH = DP / 16;                          // 16-code chunks of a row
     constexpr float U = MASK ? kLog2e : 1.f, RAISE = MASK ? 4.f : 6.f;
-    constexpr int kO = 256, kP2 = kO + 128;              // tensor-memory columns of O, of the weights' second parts; S at 0, 128
+    constexpr int kO = 256;                              // tensor-memory column of O; S buffers at 0 and 128
     extern __shared__ __align__(1024) uint8_t smem_raw[];        // the swizzle's period
     const uint32_t base = smem_u32(smem_raw);
-    const uint32_t qs = base, ks = qs + QT * PARTS * Z::tile, vs = ks + 2 * Z::tile, raw = vs + 2 * Z::tile;
+    const uint32_t qs = base, ks = qs + QT * Z::tile, vs = ks + 2 * Z::tile, raw = vs + 2 * Z::tile;
     float *share = reinterpret_cast<float *>(smem_raw + (raw + 2 * Z::raw - smem_u32(smem_raw)));     // [QT][2][128]
     const uint32_t bars = raw + 2 * Z::raw + Z::share;
     const uint32_t q_full = bars, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16, k_full = o_full + 16,
@@ -174,22 +174,13 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
                 if (!ok || d >= D) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] = 0.f;
-                } else if constexpr (BF16) {
+                } else {
                     const uint4 v = ld_nc_v4(static_cast<const uint16_t *>(p.q) + qo + d);
                     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         x[2 * e] = __uint_as_float(w[e] << 16);
                         x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-                    }
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const uint4 v = ld_nc_v4(static_cast<const float *>(p.q) + qo + d + 4 * k);
-                        x[4 * k] = __uint_as_float(v.x);
-                        x[4 * k + 1] = __uint_as_float(v.y);
-                        x[4 * k + 2] = __uint_as_float(v.z);
-                        x[4 * k + 3] = __uint_as_float(v.w);
                     }
                 }
             };
@@ -206,19 +197,10 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
             for (int d = hf * (DP / 2); d < (hf + 1) * (DP / 2); d += 8) {      // each thread its half of the row
                 float x[8];
                 load8(d, x);
-                uint32_t w[4], w2[4];
+                uint32_t w[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float a = x[2 * e] * fs, bb = x[2 * e + 1] * fs;
-                    w[e] = pack_h2(a, bb);
-                    if constexpr (PARTS == 2) {
-                        const float2 r = unpack_h2(w[e]);
-                        w2[e] = pack_h2(a - r.x, bb - r.y);
-                    }
-                }
-                sts_v4(qs + qt * PARTS * Z::tile + tile_off(row, d >> 3), make_uint4(w[0], w[1], w[2], w[3]));
-                if constexpr (PARTS == 2)
-                    sts_v4(qs + (qt * PARTS + 1) * Z::tile + tile_off(row, d >> 3), make_uint4(w2[0], w2[1], w2[2], w2[3]));
+                for (int e = 0; e < 4; ++e) w[e] = pack_h2(x[2 * e] * fs, x[2 * e + 1] * fs);
+                sts_v4(qs + qt * Z::tile + tile_off(row, d >> 3), make_uint4(w[0], w[1], w[2], w[3]));
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -332,16 +314,9 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
                 if (live) {
 #pragma unroll
                     for (int ch = 0; ch < 2; ++ch) {
-                        uint32_t s[32], ph[16], pw[16];
+                        uint32_t s[32], ph[16];
                         tc_ld_issue_x32(stm + 64 * hf + 32 * ch, s);
                         tc_wait_ld32(s);
-                        const auto keep = [&](int i, float w0, float w1) {
-                            ph[i] = pack_h2(w0, w1);
-                            if constexpr (PARTS == 2) {
-                                const float2 r = unpack_h2(ph[i]);
-                                pw[i] = pack_h2(w0 - r.x, w1 - r.y);
-                            }
-                        };
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
                             const float f = fk[2 * ch + g];
@@ -356,7 +331,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
                                     const float w1 = ex2(fmaf(__uint_as_float(s[16 * g + k + 1]), f, at));
                                     s0 += w0;
                                     s1 += w1;
-                                    keep(8 * g + k / 2, w0, w1);
+                                    ph[8 * g + k / 2] = pack_h2(w0, w1);
                                 }
                                 l = fmaf(s0 + s1, rv[2 * ch + g], l);
                             } else {
@@ -369,14 +344,13 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
                                     s0 += e0;
                                     s1 += e1;
                                     // a row that is not seen weighs nothing, even where its scale is NaN
-                                    keep(8 * g + k / 2, x0 == -INFINITY ? 0.f : e0 * wg, x1 == -INFINITY ? 0.f : e1 * wg);
+                                    ph[8 * g + k / 2] = pack_h2(x0 == -INFINITY ? 0.f : e0 * wg, x1 == -INFINITY ? 0.f : e1 * wg);
                                 }
                                 l += s0 + s1;
                             }
                         }
-                        // over this half's columns that have been read (the second parts of fp32 calls in their own)
+                        // over this half's columns that have been read
                         tc_st_32x32b_x16(stm + 64 * hf + 16 * ch, ph);
-                        if constexpr (PARTS == 2) tc_st_32x32b_x16(tmem + lanes + kP2 + 64 * buf + 32 * hf + 16 * ch, pw);
                     }
                     tc_wait_st();
                 }
@@ -409,7 +383,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
                     const float4 y = make_float4(__uint_as_float(v[k]) * f, __uint_as_float(v[k + 1]) * f,
                                                  __uint_as_float(v[k + 2]) * f, __uint_as_float(v[k + 3]) * f);
                     if (d < D) {
-                        if (wk.whole()) store4<BF16>(p.out, oo + d, y);
+                        if (wk.whole()) store4<true>(p.out, oo + d, y);
                         else *reinterpret_cast<float4 *>(po + d) = y;
                     }
                 }
@@ -466,25 +440,21 @@ __global__ void __launch_bounds__(TileSizes<DP, QT, PARTS>::threads, 1)
         auto qk = [&](int qt, int tile, int buf) {               // S[buf] = Q . K^T of row tile `tile`
             if (!failed) {
 #pragma unroll
-                for (int pt = 0; pt < PARTS; ++pt)
-#pragma unroll
-                    for (int kk = 0; kk < DP / 16; ++kk) {
-                        const uint32_t off = (kk >> 2) * kSub + (kk & 3) * 32;
-                        tc_mma_f16(tmem + buf * kRows, sw128_desc(qs + (qt * PARTS + pt) * Z::tile + off),
-                                   sw128_desc(ks + (tile & 1) * Z::tile + off), kIdesc<kRows, false>, (pt | kk) != 0);
-                    }
+                for (int kk = 0; kk < DP / 16; ++kk) {
+                    const uint32_t off = (kk >> 2) * kSub + (kk & 3) * 32;
+                    tc_mma_f16(tmem + buf * kRows, sw128_desc(qs + qt * Z::tile + off),
+                               sw128_desc(ks + (tile & 1) * Z::tile + off), kIdesc<kRows, false>, kk != 0);
+                }
             }
             tc_commit(s_full + 8 * buf);                         // also after a failure: keeps the others moving
         };
         auto pvp = [&](int qt, int tile, int buf, bool more) {   // O[qt] (+)= P[buf] . V of row tile `tile`
             if (!failed) {
 #pragma unroll
-                for (int pt = 0; pt < PARTS; ++pt)
-#pragma unroll
-                    for (int kk = 0; kk < kRows / 16; ++kk)
-                        tc_mma_f16_ta(tmem + kO + qt * DP, tmem + (pt ? kP2 + buf * 64 + kk * 8 : buf * kRows + (kk >> 2) * 64 + (kk & 3) * 8),
-                                      sw128_desc_mn(vs + (tile & 1) * Z::tile + kk * 2048, kSub), kIdesc<DP, true>,
-                                      more || (pt | kk) != 0);
+                for (int kk = 0; kk < kRows / 16; ++kk)          // a half's weights are over the first half of its columns
+                    tc_mma_f16_ta(tmem + kO + qt * DP, tmem + buf * kRows + (kk >> 2) * 64 + (kk & 3) * 8,
+                                  sw128_desc_mn(vs + (tile & 1) * Z::tile + kk * 2048, kSub), kIdesc<DP, true>,
+                                  more || kk != 0);
             }
             tc_commit(o_full + 8 * qt);
         };
@@ -536,11 +506,10 @@ int sms() {
     return n;
 }
 
-template <int DP, int QT, bool BF16, bool MASK>
+template <int DP, int QT, bool MASK>
 cudaError_t launch_t(const Kv8AttnParams &p, cudaStream_t s) {
-    constexpr int PARTS = BF16 ? 1 : 2;
-    using Z = TileSizes<DP, QT, PARTS>;
-    const auto k = kv8_attn_tile_kernel<DP, QT, PARTS, BF16, MASK>;
+    using Z = TileSizes<DP, QT>;
+    const auto k = kv8_attn_tile_kernel<DP, QT, MASK>;
     static const cudaError_t attr = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::smem);
     if (attr != cudaSuccess) return attr;
     CUtensorMap mk, mv;
@@ -550,27 +519,21 @@ cudaError_t launch_t(const Kv8AttnParams &p, cudaStream_t s) {
     return launch_pdl(k, dim3(sms()), dim3(Z::threads), Z::smem, s, mk, mv, p);
 }
 template <int DP, int QT>
-cudaError_t launch_q(const Kv8AttnParams &p, bool bf16, cudaStream_t s) {
-    const bool mask = p.mask != nullptr;
-    if constexpr (QT == 1) {
-        if (!bf16) return mask ? launch_t<DP, QT, false, true>(p, s) : launch_t<DP, QT, false, false>(p, s);
-    }
-    return mask ? launch_t<DP, QT, true, true>(p, s) : launch_t<DP, QT, true, false>(p, s);
+cudaError_t launch_q(const Kv8AttnParams &p, cudaStream_t s) {
+    return p.mask ? launch_t<DP, QT, true>(p, s) : launch_t<DP, QT, false>(p, s);
 }
 
 }  // namespace
 
-// query tiles a CTA takes at a time: two share the decoded rows where there are more than 128 queries (fp32
-// queries are two parts each, as large as two tiles)
-int kv8_tile_queries(int64_t queries, bool bf16) { return bf16 && queries > kRows ? 2 * kRows : kRows; }
+// query tiles a CTA takes at a time: two share the decoded rows where there are more than 128 queries
+int kv8_tile_queries(int64_t queries) { return queries > kRows ? 2 * kRows : kRows; }
 int kv8_tile_rows() { return kRows; }
 int kv8_tile_ctas() { return sms(); }
 
-cudaError_t kv8_tile_launch(const Kv8AttnParams &p, bool bf16, cudaStream_t s) {
+cudaError_t kv8_tile_launch(const Kv8AttnParams &p, cudaStream_t s) {
     const int64_t queries = static_cast<int64_t>(p.r.T) * (p.Hq / p.c.Hkv);
-    if (kv8_tile_queries(queries, bf16) == 2 * kRows)
-        return p.c.D <= 64 ? launch_q<64, 2>(p, bf16, s) : launch_q<128, 2>(p, bf16, s);
-    return p.c.D <= 64 ? launch_q<64, 1>(p, bf16, s) : launch_q<128, 1>(p, bf16, s);
+    if (kv8_tile_queries(queries) == 2 * kRows) return p.c.D <= 64 ? launch_q<64, 2>(p, s) : launch_q<128, 2>(p, s);
+    return p.c.D <= 64 ? launch_q<64, 1>(p, s) : launch_q<128, 1>(p, s);
 }
 
 }  // namespace onpu_b200
