@@ -248,7 +248,7 @@ struct Kv8Cache {
 };
 // the rows a call is about: tokens i < cnt[b] (null: T) of sequence b are cache rows pos[b] + i. A
 // sequence whose rows are not all inside the cache, or whose cnt is not in [0, T], is skipped and sets
-// bit 32 of *err.
+// bit 32 of *err (a wait that gave up: bit 1024).
 struct Kv8Rows {
     const int32_t *pos, *cnt;
     int T;

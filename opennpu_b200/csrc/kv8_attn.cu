@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __gri
         fence_proxy_async_smem();
         __syncthreads();                                       // before the stages are filled again
     }
-    if (failed && lane == 0) atomicOr(p.r.err, 64);
+    if (failed && lane == 0) atomicOr(p.r.err, 1024);
 }
 
 // ---------------------------------------------------------------- the shared segments

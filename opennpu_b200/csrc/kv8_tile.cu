@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
         tc_commit(drain);
         if (!mbar_wait_bounded(drain, 0, kWaitNs)) failed = true;
     }
-    if (failed && lane == 0) atomicOr(p.r.err, 64);
+    if (failed && lane == 0) atomicOr(p.r.err, 1024);
     tc_fence_before();
     __syncthreads();
     if (warp == Z::soft + kDec) tmem_dealloc(tmem, 512);

@@ -414,6 +414,8 @@ int check_device_err(Ctx &c) {
         else if (h & 32)
             set_err("rows outside an 8-bit KV cache (pos, cnt) or a cnt outside [0, T]; those sequences were "
                     "skipped (device status %d)", h);
+        else if (h & 1024)
+            set_err("attention over an 8-bit KV cache timed out waiting for its copies or products (device status %d)", h);
         else if (h & 8)
             set_err("an expert id was out of range [0, E) in a routed job list; those (token, slot) pairs were "
                     "dropped (device status %d)", h);

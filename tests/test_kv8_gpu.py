@@ -501,6 +501,50 @@ def test_decode_loop_in_a_replayed_graph_matches_eager_calls():
     assert status() == 0
 
 
+FIRST_CALL_CAPTURED = """
+import torch
+from opennpu_b200 import libonpu as L
+from opennpu_b200.kv8 import KVCache8
+c = KVCache8(2, 2, 300, 128)
+pos = torch.tensor([0, 90], dtype=torch.int32, device="cuda")
+x = torch.randn(2, 100, 12, 128, device="cuda").bfloat16()
+f = x[:, :3].float()
+outs = []
+def step():
+    c.append(x[:, :, 8:10], x[:, :, 10:], pos)
+    outs[:] = [c.attn(x[:, :, :8], pos), c.attn(f[:, :, :8], pos), *c.read(pos, tokens=100)]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    step()
+g.replay()
+got = [t.clone() for t in outs]
+step()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(got, outs))
+assert L.load().onpu_check_device() == 0
+"""
+
+
+def test_first_calls_may_be_captured():
+    """In a fresh process: the first calls of every kind inside a capture, replayed, equal eager ones."""
+    import subprocess
+    import sys
+
+    from tests.conftest import ROOT
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_calls_without_tokens():
+    c = KVCache8(2, 2, 64, 64)
+    x, pos = torch.zeros(2, 0, 2, 64, device="cuda"), i32([5, 64])
+    c.append(x, x, pos)
+    assert c.attn(x, pos).shape == x.shape and c.read(pos, tokens=0)[0].shape == x.shape
+    y = torch.full((2, 3, 4, 64), 7.0, device="cuda")
+    c.attn(y, pos, i32([0, 0]), out=y)
+    assert (y == 7).all() and status() == 0
+
+
 def test_two_graphs_and_an_eager_call_at_once_do_not_share_workspace():
     """Two captured calls replayed on two streams while a third runs eagerly on its own stream: each
     gives what it gives alone."""
