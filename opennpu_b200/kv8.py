@@ -82,7 +82,7 @@ class KVCache8:
             sb, st, sh, sd = t.stride()
         except ValueError:
             raise L.OnpuError(f"{name}: [B, T, heads, dim]") from None
-        if B != self.batch or D != self.dim or H != heads or t.get_device() != self._dev or \
+        if B != self.batch or D != self.dim or (H != heads and heads) or t.get_device() != self._dev or \
                 (t.dtype is not torch.bfloat16 and t.dtype is not torch.float32):
             raise L.OnpuError(f"{name}: bf16 or fp32 [B, T, heads, dim] on the cache's device")
         if sd != 1 or (sh != D and H > 1) or (B > 1 and T > 1 and sb != st * T):
@@ -136,9 +136,9 @@ class KVCache8:
         scale defaults to dim ** -0.5. Returns [B, T, Hq, dim] of q's type; a token whose mask leaves no
         row gets zeros, tokens at and past cnt are left as they were (undefined in a new tensor)."""
         p, n = self._places(pos, cnt)
-        Hq = q.shape[2] if q.dim() == 4 else 0
-        ldq = self._tokens(q, Hq, "q")
-        B, T, D, dev, bf16 = self.batch, q.shape[1], self.dim, self._dev, q.dtype is torch.bfloat16
+        ldq = self._tokens(q, None, "q")
+        B, T, Hq, D = q.shape
+        dev, bf16 = self._dev, q.dtype is torch.bfloat16
         mp, mbs, mts, sp = None, 0, 0, None
         if mask is not None:
             if mask.dtype is not torch.float32 or mask.dim() != 3 or mask.shape[0] not in (1, B) or \
@@ -158,12 +158,12 @@ class KVCache8:
             size = L.check(self._lib.onpu_kv8_attn_ws(self._ref, Hq, T, bf16), "onpu_kv8_attn_ws")
             self._ws[Hq, T, bf16] = size
         if stream is None:
-            ws = torch.empty(size, dtype=torch.uint8, device=self.device)
-            out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=self.device) if out is None else out
+            ws = self.k.new_empty(size)
+            out = q.new_empty(q.shape) if out is None else out
         else:
             with torch.cuda.stream(stream):        # memory that this stream may use again
-                ws = torch.empty(size, dtype=torch.uint8, device=self.device)
-                out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=self.device) if out is None else out
+                ws = self.k.new_empty(size)
+                out = q.new_empty(q.shape) if out is None else out
         ldo = self._tokens(out, Hq, "out")
         if out.shape[1] != T or out.dtype is not q.dtype:
             raise L.OnpuError("out: q's tokens and type")
