@@ -19,7 +19,7 @@
 // QT = 2 query tiles share a decoded row tile and alternate: one's softmax runs beside the other's products. QT = 1
 // (at most 128 queries) alternates two S buffers instead.
 //
-// Measured: 512 tokens over 16.8k rows, 40 query heads on 8 kv heads of 128: 254 us (0.41 of the products' floor at the
+// Measured: 512 tokens over 16.8k rows, 40 query heads on 8 kv heads of 128: 255 to 261 us (0.41 of the products' floor at the
 // measured bf16 rate; 1088 us in the kernel for few queries). With the work of a role left out, the same call takes 118 us
 // without any, 185 with the products alone, 209 with the decoding too: what is left besides the products is the chain from
 // one role to the next, several times per 128 rows, and the softmax's part of it. 128 columns a softmax thread: 280 to 298;
