@@ -269,6 +269,16 @@ __device__ __forceinline__ float out_factor(float M, float Lsum, const float *si
     return total == 0.f ? 0.f : 1.f / total;
 }
 
+// (host) SMs of the current device
+inline int kv8_sms() {
+    static const int n = [] {
+        int dev = 0, v = 0;
+        cudaGetDevice(&dev);
+        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
+        return v > 0 ? v : 1;
+    }();
+    return n;
+}
 // (host) a map of [batch][heads][rows][dim] codes whose boxes are `rows` rows of at most 128 codes, their 16-byte
 // chunks exchanged by `swizzle`; columns and rows past the ends read 0
 inline bool kv8_code_map(CUtensorMap &map, const Kv8Cache &c, int8_t *codes, int DP, int rows, CUtensorMapSwizzle swizzle) {

@@ -639,16 +639,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_rows_kernel(con
 }
 
 // ---------------------------------------------------------------- host side
-int device_sms() {
-    static const int n = [] {
-        int dev = 0, v = 0;
-        cudaGetDevice(&dev);
-        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
-        return v > 0 ? v : 1;
-    }();
-    return n;
-}
-
 // Query tiles: 8 NT queries; larger ones share the decoded codes and are limited by registers (the queries'
 // digits take 3 DP / 16 * NT, the outputs DP / 4 * NT of them).
 int pick_nt(int DP, int64_t queries) {
@@ -690,7 +680,7 @@ struct Split {
             if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
                 cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, k, kWarps * 32, smem) != cudaSuccess || per < 1)
                 per = 1;
-            return per * device_sms();
+            return per * kv8_sms();
         }();
         return n;
     }

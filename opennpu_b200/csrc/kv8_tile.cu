@@ -496,16 +496,6 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
     if (warp == Z::soft + kDec) tmem_dealloc(tmem, 512);
 }
 
-int sms() {
-    static const int n = [] {
-        int dev = 0, v = 0;
-        cudaGetDevice(&dev);
-        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
-        return v > 0 ? v : 1;
-    }();
-    return n;
-}
-
 template <int DP, int QT, bool MASK>
 cudaError_t launch_t(const Kv8AttnParams &p, cudaStream_t s) {
     using Z = TileSizes<DP, QT>;
@@ -516,7 +506,7 @@ cudaError_t launch_t(const Kv8AttnParams &p, cudaStream_t s) {
     if (!kv8_code_map(mk, p.c, p.c.k, DP, kRows, CU_TENSOR_MAP_SWIZZLE_NONE) ||
         !kv8_code_map(mv, p.c, p.c.v, DP, kRows, CU_TENSOR_MAP_SWIZZLE_NONE))
         return cudaErrorInvalidValue;
-    return launch_pdl(k, dim3(sms()), dim3(Z::threads), Z::smem, s, mk, mv, p);
+    return launch_pdl(k, dim3(kv8_sms()), dim3(Z::threads), Z::smem, s, mk, mv, p);
 }
 template <int DP, int QT>
 cudaError_t launch_q(const Kv8AttnParams &p, cudaStream_t s) {
@@ -528,7 +518,7 @@ cudaError_t launch_q(const Kv8AttnParams &p, cudaStream_t s) {
 // query tiles a CTA takes at a time: two share the decoded rows where there are more than 128 queries
 int kv8_tile_queries(int64_t queries) { return queries > kRows ? 2 * kRows : kRows; }
 int kv8_tile_rows() { return kRows; }
-int kv8_tile_ctas() { return sms(); }
+int kv8_tile_ctas() { return kv8_sms(); }
 
 cudaError_t kv8_tile_launch(const Kv8AttnParams &p, cudaStream_t s) {
     const int64_t queries = static_cast<int64_t>(p.r.T) * (p.Hq / p.c.Hkv);
