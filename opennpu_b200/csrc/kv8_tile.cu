@@ -150,6 +150,12 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
         float *mine = share + (qt * 2 + hf) * kRows + row, *other = share + (qt * 2 + (hf ^ 1)) * kRows + row;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t otm = tmem + lanes + kO + qt * DP;
+        // Product i of this query tile with V is done. QT = 1: product i - 1 may still run while the scores behind it are
+        // worked on, so odd and even products have a barrier each; one parity would not tell i from i - 2.
+        const auto wait_o = [&](int i) {
+            return QT == 2 ? mbar_wait_bounded(o_full + 8 * qt, i & 1, kWaitNs)
+                           : mbar_wait_bounded(o_full + 8 * (i & 1), i >> 1 & 1, kWaitNs);
+        };
         int pv = 0;                                      // products of this query tile with V so far
         int ns = 0;                                      // its S tiles so far
         for (; wk.segment(p, pl); wk.next()) {
@@ -226,8 +232,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                 // O times a, once its last product is done: this half of its columns
                 const auto rescale_o = [&](float a) {
                     if (j == 0 || !live) return;                 // O begins with this tile
-                    if (!failed)
-                        failed = __any_sync(0xffffffffu, !mbar_wait_bounded(o_full + 8 * qt, (pv - 1) & 1, kWaitNs));
+                    if (!failed) failed = __any_sync(0xffffffffu, !wait_o(pv - 1));
                     tc_fence_after();
 #pragma unroll 1
                     for (int ch = hf * (DP / 32); ch < (hf + 1) * (DP / 32); ++ch) {
@@ -359,7 +364,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                 if (lane == 0) mbar_arrive(p_full + 8 * buf);
                 ++pv;
             }
-            if (!failed) failed = __any_sync(0xffffffffu, !mbar_wait_bounded(o_full + 8 * qt, (pv - 1) & 1, kWaitNs));
+            if (!failed) failed = __any_sync(0xffffffffu, !wait_o(pv - 1));
             tc_fence_after();
             *mine = l;
             named_bar_sync(2 + qt, 256);
@@ -456,7 +461,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                                   sw128_desc_mn(vs + (tile & 1) * Z::tile + kk * 2048, kSub), kIdesc<DP, true>,
                                   more || kk != 0);
             }
-            tc_commit(o_full + 8 * qt);
+            tc_commit(o_full + 8 * (QT == 2 ? qt : tile & 1));
         };
         int nq[2] = {0, 0}, np[2] = {0, 0};                      // phases of q_full and p_full waited for
         for (; wk.segment(p, pl); wk.next()) {

@@ -1,0 +1,104 @@
+"""8-bit KV cache attention over long runs of rows and wide ranges of scales, against the definition in float64 for
+chosen queries: every warp and CTA takes many steps, so sums are rescaled, stages come round, and rows that a query does
+not see or hardly weighs stand beside those it does.
+
+Bounds, with p_j the query's normalised weights, A_d = sum_j p_j |v_jd| (only rows that weigh anything count), n its rows and
+big the largest sum |q_d k_d| scale over them:
+  * a score is off by big (D 2^-23 + 2^-21) (D exact products summed in fp32, possibly cut off; 22 bits of the query), e^x by
+    that plus 2^-20; numerator (A_d) and sum (|out|) both have it;
+  * adding n terms in 16-row steps, possibly cut off: (n / 16 + 64) 2^-23 A_d;
+  * fp16 weights: 2^-11 of each (A_d) for bf16 calls, 2^-21 for the two parts of fp32 calls; at most 2^-30 of the largest weight
+    for those that are tiny beside it, 127 max_j(p_j s_j) n 2^-30 in all;
+  * scales as powers of two in the exponent (bf16, many queries): logarithms up to 2^8 to 24 bits, a handful of them, 2^-13;
+  * the output's own rounding, 2^-8 or 2^-24 of it."""
+import numpy as np
+import pytest
+import torch
+
+from opennpu_b200 import libonpu as L
+from opennpu_b200.kv8 import KVCache8
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "fp32": torch.float32}
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def i32(a):
+    return torch.tensor(list(a), dtype=torch.int32, device="cuda")
+
+
+def status():
+    torch.cuda.synchronize()
+    return L.load().onpu_check_device()
+
+
+def rand_cache(rng, B, H, S, D, block):
+    codes = [np.clip(np.rint(rng.normal(size=(B, H, S, D)) * 36), -127, 127).astype(np.int8) for _ in range(2)]
+    scales = [rng.uniform(0.018, 0.038, (B, H, -(-S // block))).astype(np.float32) for _ in range(2)]
+    return [*codes, *scales]
+
+
+def rand_q(rng, shape, dtype):
+    t = torch.from_numpy(rng.normal(size=shape).astype(np.float32)).to(DT[dtype])
+    return t.float().numpy(), t.cuda()
+
+
+def attend(cache, block, b, i, h, q, pos, bf16, mask=None, sinks=None):
+    """One query's output in float64 and its bound."""
+    k, v, ks, vs = cache
+    Hq, D = q.shape[2:]
+    g = h // (Hq // k.shape[1])
+    n = int(pos[b]) + i + 1
+    m = np.zeros(n) if mask is None else np.broadcast_to(mask, (len(pos), q.shape[1], k.shape[2]))[b, i, :n].astype(np.float64)
+    rows = np.flatnonzero(~np.isneginf(m))
+    if not len(rows):
+        return np.zeros(D), np.zeros(D), n
+    s_k, s_v = (a[b, g].astype(np.float64)[rows // block] for a in (ks, vs))
+    K, V = k[b, g, rows].astype(np.float64), v[b, g, rows].astype(np.float64)
+    qv = q[b, i, h].astype(np.float64)
+    x = (K @ qv) * s_k * D ** -0.5 + m[rows]
+    big = ((np.abs(K) @ np.abs(qv)) * s_k).max() * D ** -0.5
+    top = max(x.max(), -np.inf if sinks is None else float(sinks[h]))
+    p = np.exp(x - top)
+    p /= p.sum() + (0.0 if sinks is None else np.exp(float(sinks[h]) - top))
+    w = p * s_v
+    out, A = w @ V, w @ np.abs(V)
+    d = big * (D * 2.0 ** -23 + 2.0 ** -21) + 2.0 ** -20
+    tol = A * (d + (n / 16 + 64) * 2.0 ** -23 + (2.0 ** -11 + 2.0 ** -13 if bf16 else 2.0 ** -21)) + np.abs(out) * (
+        d + (2.0 ** -8 if bf16 else 2.0 ** -23)) + 127 * w.max() * n * 2.0 ** -30
+    return out, tol, n
+
+
+def check(y, cache, block, queries, q, pos, dtype, mask=None, sinks=None):
+    """The listed (b, i, h) of y against the definition."""
+    y = y.double().cpu().numpy()
+    for b, i, h in queries:
+        out, tol, n = attend(cache, block, b, i, h, q, pos, dtype == "bf16", mask, sinks)
+        err = np.abs(y[b, i, h] - out)
+        assert (err <= tol).all(), (b, i, h, n, float((err / np.maximum(tol, 1e-300)).max()))
+
+
+def sawtooth(n, tile_blocks, step, period):
+    """Scales of n blocks: times 2^step from one run of tile_blocks to the next, back after `period` runs."""
+    return (0.02 * 2.0 ** (step * (np.arange(n) // tile_blocks % period))).astype(np.float32)
+
+
+# ---------------------------------------------------------------- sums rescaled while products run
+@pytest.mark.parametrize("D,T,step", [(128, 20, 3), (64, 32, 2), (112, 17, 5)])
+def test_value_scales_that_grow_from_tile_to_tile_at_65_to_128_queries(D, T, step):
+    """One query tile a kv head, several row tiles a CTA: the sums over the values are rescaled in most of them."""
+    H, rep, S, block = 2, 4, 37900, 32
+    rng = np.random.default_rng(D)
+    cache = rand_cache(rng, 1, H, S, D, block)
+    cache[3][:] = sawtooth(cache[3].shape[2], 128 // block, step, 8)
+    q, qt = rand_q(rng, (1, T, H * rep, D), "bf16")
+    c = KVCache8.from_tensors(*(dev(a) for a in cache), block)
+    pos = [S - T]
+    queries = [(0, 0, 0), (0, T // 2, 5), (0, T - 1, H * rep - 1)]
+    for _ in range(10):
+        y = c.attn(qt, i32(pos))
+    check(y, cache, block, queries, q, pos, "bf16")
+    assert status() == 0
