@@ -242,6 +242,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                         for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * a);
                         tc_st_32x32b_x16(otm + 16 * ch, v);
                     }
+                    tc_wait_st();                                // a second rescaling of the same tile loads what this one stored
                 };
                 if (vmax * cv > 512.f || (cv == 0.f && vmax > 0.f)) {
                     const float cn = pow2_to(vmax, 7);

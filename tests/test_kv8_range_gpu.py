@@ -102,3 +102,21 @@ def test_value_scales_that_grow_from_tile_to_tile_at_65_to_128_queries(D, T, ste
         y = c.attn(qt, i32(pos))
     check(y, cache, block, queries, q, pos, "bf16")
     assert status() == 0
+
+
+@pytest.mark.parametrize("D,T", [(128, 20), (64, 20), (128, 60)])
+def test_scores_and_value_scales_that_grow_in_the_same_tile(D, T):
+    """Both reasons to rescale a tile's sums at once: its scores pass the reference by more than 2^6, and its value scales the
+    weights' range, in tile after tile of a CTA's run."""
+    H, rep, S, block = 2, 4, 37900, 32
+    rng = np.random.default_rng(D + T)
+    cache = rand_cache(rng, 1, H, S, D, block)
+    cache[3][:] = sawtooth(cache[3].shape[2], 128 // block, 3, 8)
+    tile = np.arange(S) // 128 % 8
+    q = np.abs(rand_q(rng, (1, T, H * rep, D), "bf16")[0])
+    cache[0][:] = (18 * tile[:, None]).astype(np.int8)
+    c = KVCache8.from_tensors(*(dev(a) for a in cache), block)
+    qt = torch.from_numpy(q).to(torch.bfloat16).cuda()
+    y = c.attn(qt, i32([S - T]))
+    check(y, cache, block, [(0, 0, 0), (0, T // 2, 5), (0, T - 1, H * rep - 1)], q, [S - T], "bf16")
+    assert status() == 0
