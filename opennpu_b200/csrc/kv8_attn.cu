@@ -255,10 +255,18 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __gri
             }
         };
         load_mask(warp);
-        for (int s = warp; s < nstep; s += kWarps) {
+        for (int s = warp; s < nstep && !failed; s += kWarps) {
             __syncwarp();                                      // every lane is past its reads of the stage refilled here
             issue(s + (NS - 1) * kWarps);
-            if (!failed) failed = __any_sync(0xffffffffu, !mbar_wait_bounded(bar0 + 8 * stage, parity, kWaitNs));
+            failed = __any_sync(0xffffffffu, !mbar_wait_bounded(bar0 + 8 * stage, parity, kWaitNs));
+            if (failed) {                                      // no more steps; the copies in flight, this one first, once more
+                do {
+                    mbar_wait_bounded(bar0 + 8 * stage, parity, kWaitNs);
+                    stage = stage + 1 == NS ? 0 : stage + 1;
+                    parity ^= stage == 0;
+                } while (stage != filled);
+                break;
+            }
             const uint32_t kb = wbase + stage * STB, vb = kb + DP * ROWS;
             stage = stage + 1 == NS ? 0 : stage + 1;
             parity ^= stage == 0;
@@ -435,12 +443,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __gri
                     }
                 }
         }
-        // merge the warps in shared memory: every copy has been waited for (after a failure, once more)
-        if (failed)
-            for (; stage != filled; stage = stage + 1 == NS ? 0 : stage + 1) {
-                mbar_wait_bounded(bar0 + 8 * stage, parity, kWaitNs);
-                parity ^= stage + 1 == NS;
-            }
+        // merge the warps in shared memory: every copy has been waited for
         __syncthreads();
         float *osm = reinterpret_cast<float *>(smem);                              // [warps][8 NT][DP + 4]
         float2 *msm = reinterpret_cast<float2 *>(osm + kWarps * 8 * NT * (DP + 4));    // [warps][8 NT] reference, sum

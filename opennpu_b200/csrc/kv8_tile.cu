@@ -401,6 +401,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
     } else if (warp < Z::soft + kDec) {
         // ============================================================ decode
         const int dt = threadIdx.x - Z::soft * 32;
+        unsigned fetched = 0;                                    // bit 0, 1: the parity of thread 0's copies of K, V so far
         for (; wk.segment(p, pl); wk.next()) {
             const int row0 = wk.ua * kRows, n = wk.ub - wk.ua;
             const auto fetch = [&](int kv, int j) {              // codes of row tile j of K or V
@@ -408,6 +409,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                 const uint32_t bar = raw_full + 8 * kv;
                 mbar_arrive_expect_tx(bar, Z::raw);
                 tma_codes(raw + kv * Z::raw, kv ? &mapv : &mapk, row0 + j * kRows, wk.h, wk.b, bar);
+                fetched ^= 1u << kv;
             };
             fetch(0, 0);
             fetch(1, 0);
@@ -435,8 +437,9 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                 }
             }
         }
-        if (failed && dt == 0)                                   // copies in flight land before the CTA ends
-            for (int kv = 0; kv < 2; ++kv) mbar_wait_bounded(raw_full + 8 * kv, jt & 1, kWaitNs);
+        if (failed && dt == 0)                                   // copies in flight, the last of each, land before the CTA ends
+            for (int kv = 0; kv < 2; ++kv)
+                mbar_wait_bounded(raw_full + 8 * kv, ~(fetched >> kv) & 1, kWaitNs);
     } else if (lane == 0) {
         // ============================================================ products
         auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -496,7 +499,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
         tc_commit(drain);
         if (!mbar_wait_bounded(drain, 0, kWaitNs)) failed = true;
     }
-    if (failed && lane == 0) atomicOr(p.r.err, 1024);
+    if (failed) atomicOr(p.r.err, 1024);
     tc_fence_before();
     __syncthreads();
     if (warp == Z::soft + kDec) tmem_dealloc(tmem, 512);
