@@ -409,7 +409,8 @@ typedef struct onpu_kv8_cache {
  * grow; cnt NULL: T everywhere; cnt[b] = 0 leaves sequence b alone. Token rows (k, v, q, out) lie at
  * (b * T + i) * ld, heads one after another in a row; rows i >= cnt[b] of a padded batch are neither
  * read nor written. They are bf16 (x_bf16 != 0) or fp32, 16-byte aligned, ld times the element a
- * multiple of 16 bytes. dim is a multiple of 16, at most 256; batch at most 32767. A sequence whose rows are
+ * multiple of 16 bytes; pos, cnt, mask and sinks are 4-byte aligned. dim is a multiple of 16, at most 256; batch at
+ * most 32767. A sequence whose rows are
  * not all inside the cache, or whose cnt is not in [0, T], is skipped and sets the device status
  * (onpu_check_device). Asynchronous on `stream`, no allocation, capturable; calls that touch the same
  * sequence's rows are ordered by the caller, and pos and cnt stay as they are until a call is done. The device that is current must be the library's.

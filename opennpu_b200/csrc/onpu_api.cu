@@ -2745,6 +2745,10 @@ bool kv8_check(const char *who, const onpu_kv8_cache *d, int64_t T, const int32_
         set_err("%s: a null cache, codes, scales or pos pointer", who);
         return false;
     }
+    if ((reinterpret_cast<uintptr_t>(pos) | reinterpret_cast<uintptr_t>(cnt)) & 3) {
+        set_err("%s: pos and cnt must be 4-byte aligned", who);
+        return false;
+    }
     if (d->batch < 1 || d->batch > 32767 || d->heads < 1 || d->heads > 65535 || d->rows < 1 || d->rows > 0x7fffff00 ||
         d->dim < 16 || d->dim > 256 || d->dim % 16 || (d->block != 16 && d->block != 32 && d->block != 64)) {
         set_err("%s: need 1 <= batch <= 32767, 1 <= heads <= 65535, 1 <= rows <= 2^31 - 256, dim a multiple of 16 up to "
@@ -2873,6 +2877,10 @@ int onpu_kv8_attn_dev(const onpu_kv8_cache *cache, const void *q, int64_t ldq, i
         return -1;
     if (!ws || (reinterpret_cast<uintptr_t>(ws) & 15)) {
         set_err("%s: ws must be 16-byte aligned device memory of onpu_kv8_attn_ws bytes", who);
+        return -1;
+    }
+    if ((reinterpret_cast<uintptr_t>(mask) | reinterpret_cast<uintptr_t>(sinks)) & 3) {
+        set_err("%s: mask and sinks must be 4-byte aligned", who);
         return -1;
     }
     if (!kv8_device(who, p.r)) return -1;
