@@ -17,7 +17,8 @@ def _need(ok, what):
 class KVCache8:
     """B sequences of up to ``rows`` rows, ``heads`` kv heads of ``dim`` (a multiple of 16, at most 256),
     ``block`` (16, 32 or 64) rows to a scale. ``k``, ``v``: int8 [B, heads, rows, dim]; ``k_scale``,
-    ``v_scale``: fp32 [B, heads, ceil(rows / block)].
+    ``v_scale``: fp32 [B, heads, ceil(rows / block)]. All on the library's device, which has to be the current
+    one, in the calls too.
 
     The calls take, for T tokens of each sequence, ``pos`` (int32 CUDA [B]): the cache row of a
     sequence's first token, and ``cnt`` (int32 CUDA [B], or None for T everywhere): how many of its T
@@ -48,6 +49,8 @@ class KVCache8:
               "v: like k, with the same strides")
         B, H, S, D = k.shape
         _need(block in (16, 32, 64), "block: 16, 32 or 64")
+        # the library runs on the device that is current here (onpu_kv8_attn_ws below checks that it is its own)
+        _need(k.get_device() == torch.cuda.current_device(), "k: on the current device")
         nb = -(-S // block)
         for t in (k_scale, v_scale):
             _need(t.dtype == torch.float32 and t.shape == (B, H, nb) and t.device == k.device and

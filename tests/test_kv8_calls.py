@@ -1,8 +1,10 @@
-"""What the 8-bit KV cache's entries refuse before any device call: pointers that a kernel could not read."""
+"""What the 8-bit KV cache's entries and wrapper refuse before any device call: addresses that a kernel could not read."""
 import ctypes as C
 
 import pytest
+import torch
 
+from opennpu_b200 import kv8
 from opennpu_b200 import libonpu as L
 
 DESC = L.Kv8Cache(1 << 20, 1 << 21, 1 << 22, 1 << 23, 2, 4, 100, 64, 4 * 100 * 64, 100 * 64, 64, 16, 4, 32)
@@ -23,3 +25,33 @@ def call(fn, pos=POS, cnt=None, mask=None, sinks=None):
 def test_words_that_are_not_4_byte_aligned_are_refused(fn, bad):
     assert call(fn, **{bad: ODD}) < 0
     assert f"onpu_kv8_{fn}_dev" in L.last_error() and "4-byte aligned" in L.last_error()
+
+
+class FakeCuda:
+    """What the wrapper looks at of a dense CUDA tensor on device 1."""
+    is_cuda, device = True, torch.device("cuda", 1)
+
+    def __init__(self, dtype, *shape):
+        self.dtype, self.shape = dtype, torch.Size(shape)
+
+    def dim(self):
+        return len(self.shape)
+
+    def stride(self, i=None):
+        s = torch.empty(self.shape, device="meta").stride()
+        return s if i is None else s[i]
+
+    def get_device(self):
+        return 1
+
+    def data_ptr(self):
+        return 1 << 20
+
+
+def test_a_cache_on_another_device_than_the_current_one_is_refused(monkeypatch):
+    """The kernels run on the library's device, which the current one has to be, and would read the cache's addresses there."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(L, "require_device", lambda: pytest.fail("the cache was taken"))
+    k, s = FakeCuda(torch.int8, 2, 4, 100, 64), FakeCuda(torch.float32, 2, 4, 4)
+    with pytest.raises(L.OnpuError, match="current device"):
+        kv8.KVCache8.from_tensors(k, k, s, s)
