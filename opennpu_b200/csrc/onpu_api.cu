@@ -15,6 +15,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <functional>
 #include <map>
 #include <mutex>
 #include <set>
@@ -80,7 +81,7 @@ bool grow(T *&p, int64_t &cap, int64_t n, bool zero = false) {
 }
 
 struct Ctx {
-    bool tried = false, ok = false;
+    bool ok = false;
     int device = 0, nsm = 0;
     cudaStream_t stream = nullptr;
     int *d_err = nullptr;
@@ -136,29 +137,30 @@ struct Ctx {
     int64_t gemv_trace_ctas = 0;
 };
 
+void ctx_init(Ctx &c) {
+    int n = 0;
+    if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
+        cudaGetLastError();
+        return;
+    }
+    if (cudaGetDevice(&c.device) != cudaSuccess) return;
+    cudaDeviceProp prop;
+    if (cudaGetDeviceProperties(&prop, c.device) != cudaSuccess) return;
+    c.nsm = prop.multiProcessorCount;
+    if (prop.major < 10) {
+        fprintf(stderr, "onpu: %s (sm_%d%d) is not a B200-class GPU; libonpu targets sm_100a\n", prop.name,
+                prop.major, prop.minor);
+        return;
+    }
+    if (cudaStreamCreateWithFlags(&c.stream, cudaStreamNonBlocking) != cudaSuccess) return;
+    if (cudaMalloc(&c.d_err, sizeof(int)) != cudaSuccess) return;
+    cudaMemset(c.d_err, 0, sizeof(int));
+    c.ok = true;
+}
 Ctx &ctx() {
     static Ctx c;
-    if (!c.tried) {
-        c.tried = true;
-        int n = 0;
-        if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
-            cudaGetLastError();
-            return c;
-        }
-        if (cudaGetDevice(&c.device) != cudaSuccess) return c;
-        cudaDeviceProp prop;
-        if (cudaGetDeviceProperties(&prop, c.device) != cudaSuccess) return c;
-        c.nsm = prop.multiProcessorCount;
-        if (prop.major < 10) {
-            fprintf(stderr, "onpu: %s (sm_%d%d) is not a B200-class GPU; libonpu targets sm_100a\n", prop.name,
-                    prop.major, prop.minor);
-            return c;
-        }
-        if (cudaStreamCreateWithFlags(&c.stream, cudaStreamNonBlocking) != cudaSuccess) return c;
-        if (cudaMalloc(&c.d_err, sizeof(int)) != cudaSuccess) return c;
-        cudaMemset(c.d_err, 0, sizeof(int));
-        c.ok = true;
-    }
+    static std::once_flag once;        // entries that take no lock may be several threads' first calls
+    std::call_once(once, ctx_init, std::ref(c));
     return c;
 }
 

@@ -120,3 +120,48 @@ def test_scores_and_value_scales_that_grow_in_the_same_tile(D, T):
     y = c.attn(qt, i32([S - T]))
     check(y, cache, block, [(0, 0, 0), (0, T // 2, 5), (0, T - 1, H * rep - 1)], q, [S - T], "bf16")
     assert status() == 0
+
+
+# ---------------------------------------------------------------- calls of several threads
+FIRST_CALLS_AT_ONCE = """
+import threading
+import torch
+from opennpu_b200 import libonpu as L
+from opennpu_b200.kv8 import KVCache8
+N = 16
+L.load()
+pos = torch.zeros(1, dtype=torch.int32, device="cuda")
+x = torch.randn(1, 40, 12, 128, device="cuda").bfloat16()
+torch.cuda.synchronize()
+starts, caches, outs, errors = [threading.Barrier(N) for _ in range(3)], [None] * N, [None] * N, []
+def work(i):
+    try:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            starts[0].wait()
+            c = caches[i] = KVCache8(1, 2, 300, 128)
+            starts[1].wait()
+            c.append(x[:, :, 8:10], x[:, :, 10:], pos)
+            starts[2].wait()
+            outs[i] = c.attn(x[:, :40 if i % 2 else 1, :8], pos)
+            torch.cuda.current_stream().synchronize()
+    except Exception as e:
+        errors.append(repr(e))
+        [s.abort() for s in starts]
+threads = [threading.Thread(target=work, args=(i,)) for i in range(N)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert not errors, errors
+assert all(torch.equal(outs[i], outs[i % 2]) for i in range(N))
+assert L.load().onpu_check_device() == 0
+"""
+
+
+def test_first_calls_of_several_threads_at_once():
+    """In a fresh process: what the library looks up in a first call is there for the calls beside it."""
+    import subprocess
+    import sys
+
+    from tests.conftest import ROOT
+    for _ in range(3):
+        r = subprocess.run([sys.executable, "-c", FIRST_CALLS_AT_ONCE], cwd=ROOT, capture_output=True, text=True, timeout=300)
+        assert r.returncode == 0, r.stderr[-2000:]
