@@ -261,8 +261,9 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                         rv[g] = __shfl_sync(0xffffffffu, iv, 8 + 4 * hf + g);
                     }
                 }
-                const bool above0 = !(lane >= 8 && lane < 16 && !(scj > 0.f));
-                const bool usual = !MASK && r0 + kRows <= edge && __all_sync(0xffffffffu, above0);
+                // (where V's scales are far apart, s_v c and the weights with it would underflow and be missing in the sum)
+                const bool near = !(lane >= 8 && lane < 16 && !(cv * scj > 0x1p-40f));
+                const bool usual = !MASK && r0 + kRows <= edge && __all_sync(0xffffffffu, near);
                 const uint32_t sphase = QT == 2 ? ns & 1 : ns >> 1 & 1;
                 if (!failed) failed = __any_sync(0xffffffffu, !mbar_wait_bounded(s_full + 8 * buf, sphase, kWaitNs));
                 ++ns;
@@ -328,7 +329,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                             const float f = fk[2 * ch + g];
                             float s0 = 0.f, s1 = 0.f;
                             if (usual) {
-                                // V's scales are above 0: a weight is one exponential, w = 2^(S f - m + log2(s_v c)), and the
+                                // V's scales are above 0 and alike: a weight is one exponential, w = 2^(S f - m + log2(s_v c)), and the
                                 // sum takes w / (s_v c)
                                 const float at = lg[2 * ch + g] - m;
 #pragma unroll

@@ -22,10 +22,6 @@ pytestmark = pytest.mark.gpu
 DT = {"bf16": torch.bfloat16, "fp32": torch.float32}
 
 
-def dev(a):
-    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
-
-
 def i32(a):
     return torch.tensor(list(a), dtype=torch.int32, device="cuda")
 
@@ -35,55 +31,63 @@ def status():
     return L.load().onpu_check_device()
 
 
-def rand_cache(rng, B, H, S, D, block):
-    codes = [np.clip(np.rint(rng.normal(size=(B, H, S, D)) * 36), -127, 127).astype(np.int8) for _ in range(2)]
-    scales = [rng.uniform(0.018, 0.038, (B, H, -(-S // block))).astype(np.float32) for _ in range(2)]
+def rand_cache(seed, B, H, S, D, block):
+    """CUDA tensors k, v, k_scale, v_scale: values of about unit size"""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    codes = [torch.randn(B, H, S, D, device="cuda", generator=g).mul_(36).round_().clamp_(-127, 127).to(torch.int8)
+             for _ in range(2)]
+    scales = [torch.rand(B, H, -(-S // block), device="cuda", generator=g) * 0.02 + 0.018 for _ in range(2)]
     return [*codes, *scales]
 
 
-def rand_q(rng, shape, dtype):
-    t = torch.from_numpy(rng.normal(size=shape).astype(np.float32)).to(DT[dtype])
-    return t.float().numpy(), t.cuda()
+def rand_q(seed, shape, dtype):
+    g = torch.Generator(device="cuda").manual_seed(seed + 1000)
+    return torch.randn(shape, device="cuda", generator=g).to(DT[dtype])
 
 
-def attend(cache, block, b, i, h, q, pos, bf16, mask=None, sinks=None):
+def attend(cache, block, b, i, h, q, pos, mask=None, sinks=None):
     """One query's output in float64 and its bound."""
     k, v, ks, vs = cache
-    Hq, D = q.shape[2:]
-    g = h // (Hq // k.shape[1])
-    n = int(pos[b]) + i + 1
-    m = np.zeros(n) if mask is None else np.broadcast_to(mask, (len(pos), q.shape[1], k.shape[2]))[b, i, :n].astype(np.float64)
-    rows = np.flatnonzero(~np.isneginf(m))
+    (T, Hq, D), bf16 = q.shape[1:], q.dtype == torch.bfloat16
+    g, n = h // (Hq // k.shape[1]), int(pos[b]) + i + 1
+    rows = torch.arange(n, device=k.device)
+    m = torch.zeros(n, dtype=torch.float64, device=k.device)
+    if mask is not None:
+        m = mask.expand(len(pos), T, k.shape[2])[b, i, :n].double()
+        rows, m = rows[m > -np.inf], m[m > -np.inf]
     if not len(rows):
-        return np.zeros(D), np.zeros(D), n
-    s_k, s_v = (a[b, g].astype(np.float64)[rows // block] for a in (ks, vs))
-    K, V = k[b, g, rows].astype(np.float64), v[b, g, rows].astype(np.float64)
-    qv = q[b, i, h].astype(np.float64)
-    x = (K @ qv) * s_k * D ** -0.5 + m[rows]
-    big = ((np.abs(K) @ np.abs(qv)) * s_k).max() * D ** -0.5
-    top = max(x.max(), -np.inf if sinks is None else float(sinks[h]))
-    p = np.exp(x - top)
-    p /= p.sum() + (0.0 if sinks is None else np.exp(float(sinks[h]) - top))
+        return torch.zeros(D, dtype=torch.float64, device=k.device), 0.0
+    s_k, s_v = (a[b, g].double()[rows // block] for a in (ks, vs))
+    K, V, qv = k[b, g, rows].double(), v[b, g, rows].double(), q[b, i, h].double()
+    x = (K @ qv) * s_k * D ** -0.5 + m
+    big = float(((K.abs() @ qv.abs()) * s_k).max()) * D ** -0.5
+    top = float(x.max()) if sinks is None else max(float(x.max()), float(sinks[h]))
+    p = torch.exp(x - top)
+    p /= p.sum() + (0.0 if sinks is None else float(torch.exp(sinks[h].double() - top)))
     w = p * s_v
-    out, A = w @ V, w @ np.abs(V)
+    out, A = w @ V, w @ V.abs()
     d = big * (D * 2.0 ** -23 + 2.0 ** -21) + 2.0 ** -20
-    tol = A * (d + (n / 16 + 64) * 2.0 ** -23 + (2.0 ** -11 + 2.0 ** -13 if bf16 else 2.0 ** -21)) + np.abs(out) * (
+    tol = A * (d + (n / 16 + 64) * 2.0 ** -23 + (2.0 ** -11 + 2.0 ** -13 if bf16 else 2.0 ** -21)) + out.abs() * (
         d + (2.0 ** -8 if bf16 else 2.0 ** -23)) + 127 * w.max() * n * 2.0 ** -30
-    return out, tol, n
+    return out, tol
 
 
-def check(y, cache, block, queries, q, pos, dtype, mask=None, sinks=None):
+def check(y, cache, block, queries, q, pos, mask=None, sinks=None):
     """The listed (b, i, h) of y against the definition."""
-    y = y.double().cpu().numpy()
     for b, i, h in queries:
-        out, tol, n = attend(cache, block, b, i, h, q, pos, dtype == "bf16", mask, sinks)
-        err = np.abs(y[b, i, h] - out)
-        assert (err <= tol).all(), (b, i, h, n, float((err / np.maximum(tol, 1e-300)).max()))
+        out, tol = attend(cache, block, b, i, h, q, pos, mask, sinks)
+        err = (y[b, i, h].double() - out).abs()
+        assert bool((err <= tol).all()), (b, i, h, int(pos[b]) + i + 1, float(err.max()), float(out.abs().max()))
 
 
 def sawtooth(n, tile_blocks, step, period):
     """Scales of n blocks: times 2^step from one run of tile_blocks to the next, back after `period` runs."""
-    return (0.02 * 2.0 ** (step * (np.arange(n) // tile_blocks % period))).astype(np.float32)
+    return 0.02 * 2.0 ** (step * (torch.arange(n, device="cuda") // tile_blocks % period)).float()
+
+
+def some_queries(B, T, Hq, count=6):
+    rng = np.random.default_rng(B + T + Hq)
+    return [(0, 0, 0), (B - 1, T - 1, Hq - 1)] + [tuple(int(rng.integers(n)) for n in (B, T, Hq)) for _ in range(count)]
 
 
 # ---------------------------------------------------------------- sums rescaled while products run
@@ -91,16 +95,13 @@ def sawtooth(n, tile_blocks, step, period):
 def test_value_scales_that_grow_from_tile_to_tile_at_65_to_128_queries(D, T, step):
     """One query tile a kv head, several row tiles a CTA: the sums over the values are rescaled in most of them."""
     H, rep, S, block = 2, 4, 37900, 32
-    rng = np.random.default_rng(D)
-    cache = rand_cache(rng, 1, H, S, D, block)
+    cache = rand_cache(D, 1, H, S, D, block)
     cache[3][:] = sawtooth(cache[3].shape[2], 128 // block, step, 8)
-    q, qt = rand_q(rng, (1, T, H * rep, D), "bf16")
-    c = KVCache8.from_tensors(*(dev(a) for a in cache), block)
-    pos = [S - T]
-    queries = [(0, 0, 0), (0, T // 2, 5), (0, T - 1, H * rep - 1)]
+    q = rand_q(D, (1, T, H * rep, D), "bf16")
+    c = KVCache8.from_tensors(*cache, block)
     for _ in range(10):
-        y = c.attn(qt, i32(pos))
-    check(y, cache, block, queries, q, pos, "bf16")
+        y = c.attn(q, i32([S - T]))
+        check(y, cache, block, some_queries(1, T, H * rep, 1), q, [S - T])
     assert status() == 0
 
 
@@ -109,16 +110,29 @@ def test_scores_and_value_scales_that_grow_in_the_same_tile(D, T):
     """Both reasons to rescale a tile's sums at once: its scores pass the reference by more than 2^6, and its value scales the
     weights' range, in tile after tile of a CTA's run."""
     H, rep, S, block = 2, 4, 37900, 32
-    rng = np.random.default_rng(D + T)
-    cache = rand_cache(rng, 1, H, S, D, block)
+    cache = rand_cache(D + T, 1, H, S, D, block)
     cache[3][:] = sawtooth(cache[3].shape[2], 128 // block, 3, 8)
-    tile = np.arange(S) // 128 % 8
-    q = np.abs(rand_q(rng, (1, T, H * rep, D), "bf16")[0])
-    cache[0][:] = (18 * tile[:, None]).astype(np.int8)
-    c = KVCache8.from_tensors(*(dev(a) for a in cache), block)
-    qt = torch.from_numpy(q).to(torch.bfloat16).cuda()
-    y = c.attn(qt, i32([S - T]))
-    check(y, cache, block, [(0, 0, 0), (0, T // 2, 5), (0, T - 1, H * rep - 1)], q, [S - T], "bf16")
+    cache[0][:] = (18 * (torch.arange(S, device="cuda") // 128 % 8))[:, None].to(torch.int8)
+    q = rand_q(D, (1, T, H * rep, D), "bf16").abs()
+    c = KVCache8.from_tensors(*cache, block)
+    y = c.attn(q, i32([S - T]))
+    check(y, cache, block, some_queries(1, T, H * rep), q, [S - T])
+    assert status() == 0
+
+
+# ---------------------------------------------------------------- value scales far apart
+@pytest.mark.parametrize("T,D", [(20, 128), (20, 64), (60, 128), (60, 64)])
+@pytest.mark.parametrize("tiny", [1e-38, 1e-41, 1e-44])
+def test_blocks_of_tiny_values_count_in_the_sum(T, D, tiny):
+    """More than 64 bf16 queries a kv head: every other block holds values near fp32's smallest, and weighs in the
+    softmax's sum like any other."""
+    H, rep, S, block = 2, 4, 37900, 32
+    cache = rand_cache(T + D, 1, H, S, D, block)
+    cache[3][:, :, 1::2] = tiny
+    q = rand_q(T, (1, T, H * rep, D), "bf16")
+    c = KVCache8.from_tensors(*cache, block)
+    y = c.attn(q, i32([S - T]))
+    check(y, cache, block, some_queries(1, T, H * rep), q, [S - T])
     assert status() == 0
 
 
