@@ -15,9 +15,10 @@
 //    decoding, and an int8 product has twice the k of an fp16 one at the same rate (4.4 ns a warp
 //    instruction on one of an SM's four quarters, both). Against fp16 q (two parts for fp32) and decoded K, with cp.async:
 //    one token over 131001 rows 65.0 -> 49.5 us, 484 warp instructions per 16 rows before.
-//  * weights: w = 2^(x - m) * s_v * c, c a power of two that keeps s_v * c below 2^9, rounded to fp16 (one
-//    part for bf16 outputs: 2^-11 of a weight against the output's 2^-8; two parts, 22 bits, for fp32), times V's codes
-//    as fp16, exactly (|c| <= 127): 0x64uu is 1024 + uu.
+//  * weights: w = 2^(x - m) * s_v * c, rounded to fp16 (one part for bf16 outputs: 2^-11 of a weight against the output's
+//    2^-8; two parts, 22 bits, for fp32), times V's codes as fp16, exactly (|c| <= 127): 0x64uu is 1024 + uu. c is a
+//    query's own and puts the largest weight that it has had at 2^6 to 2^10: what it does not see or what weighs nothing does
+//    not count, however large its s_v is. Weights 2^20 below that one (two parts: 2^9) lose bits, 2^-31 of it at most.
 //  * m is a reference within 2^6 (no mask) or e^4 (mask) of the running maximum, raised only when a score
 //    passes it by more: the accumulators are rescaled a few times a sequence, not every step. With a mask
 //    scores stay in natural units, x - m is formed first, so masks of the lowest finite value stay finite.
@@ -90,8 +91,13 @@ __device__ __forceinline__ void mma_s8u8(int (&d)[4], const uint32_t (&a)[4], ui
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// CTAs an SM that the registers are to allow; 0: the compiler's choice. For fp32 it spills to fit three: one token over 4096 rows
+// 11.0 us, 9.2 with two.
+template <int DP, int NT, bool BF16>
+constexpr int kMinCtas = DP == 128 && NT == 1 && !BF16 ? 2 : 0;
+
 template <int DP, int NT, bool BF16, bool MASK, int R, int NS>
-__global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __grid_constant__ CUtensorMap mapk,
+__global__ void __launch_bounds__(kWarps * 32, kMinCtas<DP, NT, BF16>) kv8_attn_split_kernel(const __grid_constant__ CUtensorMap mapk,
                                                                      const __grid_constant__ CUtensorMap mapv,
                                                                      const Kv8AttnParams p) {
     constexpr int PARTS = BF16 ? 1 : 2;             // fp16 parts of a weight
@@ -232,13 +238,16 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __gri
         // the first row that some query of the tile must not see (queries past nq do not matter)
         const int edge = pos + static_cast<int>(div64(q0, pl.rep)) + 1;
 
-        float o[VW * 2][NT][4], m[NT][2], l[NT][2], cv = 0.f;
+        // cw: what the weights are times, 0 before a query's first weight
+        float o[VW * 2][NT][4], m[NT][2], l[NT][2], cw[NT][2], cmax = INFINITY;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int i = 0; i < VW * 2; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
             m[nt][0] = m[nt][1] = -INFINITY;
             l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) cw[nt][k] = lim[nt][k] < 0 ? 0x1p-126f : 0.f;     // no query: nothing to set
         }
         float mk[R][NT][4];                                    // the mask of this warp's next step
         auto load_mask = [&](int s) {
@@ -328,45 +337,56 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __gri
                     for (int i = 1; i < R; ++i) mx = fmaxf(mx, fmaxf(x[i][nt][k], x[i][nt][k + 2]));
                     up |= mx > m[nt][k] + RAISE;
                 }
-            if (__any_sync(0xffffffffu, up)) {
+            float svm = sv[0];
+#pragma unroll
+            for (int i = 1; i < R; ++i) svm = fmaxf(svm, sv[i]);
+            // m and the weights' factors: looked at where a score passes m, where a weight might pass fp16's range, and while a
+            // query has had no weight (cmax is inf then)
+            if (__any_sync(0xffffffffu, up) || svm * cmax > 1000.f || cmax == INFINITY) {
+                cmax = 0.f;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        float mx = fmaxf(x[0][nt][k], x[0][nt][k + 2]);
+                        float top[R], mn = m[nt][k];           // the largest score of each 16 rows
 #pragma unroll
-                        for (int i = 1; i < R; ++i) mx = fmaxf(mx, fmaxf(x[i][nt][k], x[i][nt][k + 2]));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        const float mn = fmaxf(m[nt][k], mx);
-                        const float a = mn == -INFINITY ? 1.f : ex2((m[nt][k] - mn) * U);
-                        m[nt][k] = mn;
-                        l[nt][k] *= a;
-#pragma unroll
-                        for (int i = 0; i < VW * 2; ++i) {
-                            o[i][nt][k] *= a;
-                            o[i][nt][k + 2] *= a;
+                        for (int i = 0; i < R; ++i) {
+                            top[i] = fmaxf(x[i][nt][k], x[i][nt][k + 2]);
+                            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 4));
+                            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 8));
+                            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
+                            mn = fmaxf(mn, top[i]);
                         }
+                        float wm = 0.f;                        // the step's largest weight; rows that are not seen have none
+#pragma unroll
+                        for (int i = 0; i < R; ++i)
+                            if (top[i] != -INFINITY) wm = fmaxf(wm, ex2((top[i] - mn) * U) * sv[i]);
+                        const float by = mn == -INFINITY ? 0.f : (m[nt][k] - mn) * U, c0 = cw[nt][k];
+                        m[nt][k] = mn;
+                        l[nt][k] *= ex2(by);
+                        // m raised, the weights so far stay what they are times a larger factor; o changes with them only where
+                        // the new ones need a smaller one
+                        float cn = c0 > 0.f ? fminf(c0 * ex2(-by), 0x1p126f) : 0.f;
+                        const bool over = wm * cn > 1000.f;
+                        if (over || (c0 == 0.f && wm > 0.f)) cn = pow2_to(wm, 6);
+                        if (c0 > 0.f && (over || cn == 0x1p126f)) {        // o 2^by cn / c0, cn a power of two
+                            const int d = static_cast<int>(__float_as_uint(cn) >> 23) - static_cast<int>(__float_as_uint(c0) >> 23);
+                            const float a = __fdividef(ex2(by + d), __uint_as_float((__float_as_uint(c0) & 0x7fffffu) | 0x3f800000u));
+#pragma unroll
+                            for (int i = 0; i < VW * 2; ++i) {
+                                o[i][nt][k] *= a;
+                                o[i][nt][k + 2] *= a;
+                            }
+                        }
+                        cw[nt][k] = cn;
+                        cmax = fmaxf(cmax, cn == 0.f ? INFINITY : cn);
                     }
-            }
-            float svm = sv[0];
-#pragma unroll
-            for (int i = 1; i < R; ++i) svm = fmaxf(svm, sv[i]);
-            if (svm * cv > 512.f || (cv == 0.f && svm > 0.f)) {             // uniform: the weights' power of two
-                const float cn = pow2_to(svm, 7), a = cv == 0.f ? 1.f : cn / cv;
-                cv = cn;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int i = 0; i < VW * 2; ++i)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) o[i][nt][k] *= a;
+                cmax = fmaxf(cmax, __shfl_xor_sync(0xffffffffu, cmax, 1));
+                cmax = fmaxf(cmax, __shfl_xor_sync(0xffffffffu, cmax, 2));
             }
             uint32_t pb[R][PARTS][NT][2];
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                const float svc = sv[i] * cv;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float w[4];
@@ -375,7 +395,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __gri
                         const float mr = m[nt][k & 1] == -INFINITY ? 0.f : m[nt][k & 1];
                         const float e2 = ex2((x[i][nt][k] - mr) * U);
                         l[nt][k & 1] += e2;
-                        w[k] = e2 * svc;
+                        w[k] = e2 * sv[i] * cw[nt][k & 1];     // in this order: a large scale that hardly weighs stays finite
                         // a row that is not seen weighs nothing, even where its scale is NaN
                         if (x[i][nt][k] == -INFINITY) w[k] = 0.f;
                     }
@@ -447,11 +467,11 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attn_split_kernel(const __gri
         __syncthreads();
         float *osm = reinterpret_cast<float *>(smem);                              // [warps][8 NT][DP + 4]
         float2 *msm = reinterpret_cast<float2 *>(osm + kWarps * 8 * NT * (DP + 4));    // [warps][8 NT] reference, sum
-        const float inv = cv == 0.f ? 1.f : 1.f / cv;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
+                const float inv = cw[nt][k] == 0.f ? 1.f : __fdividef(1.f, cw[nt][k]);
                 float s = l[nt][k];
                 s += __shfl_xor_sync(0xffffffffu, s, 4);
                 s += __shfl_xor_sync(0xffffffffu, s, 8);

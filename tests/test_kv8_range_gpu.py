@@ -6,9 +6,10 @@ Bounds, with p_j the query's normalised weights, A_d = sum_j p_j |v_jd| (only ro
 big the largest sum |q_d k_d| scale over them:
   * a score is off by big (D 2^-23 + 2^-21) (D exact products summed in fp32, possibly cut off; 22 bits of the query), e^x by
     that plus 2^-20; numerator (A_d) and sum (|out|) both have it;
-  * adding n terms in 16-row steps, possibly cut off: (n / 16 + 64) 2^-23 A_d;
-  * fp16 weights: 2^-11 of each (A_d) for bf16 calls, 2^-21 for the two parts of fp32 calls; at most 2^-30 of the largest weight
-    for those that are tiny beside it, 127 max_j(p_j s_j) n 2^-30 in all;
+  * adding in 16-row steps, possibly cut off: (c / 16 + 128) 2^-23 A_d, c the rows that a CTA sums on its own, at most n: the
+    list's 128-row units over at least 148 CTAs, two more for its ends; 128 for the parts joined;
+  * fp16 weights: 2^-11 of each (A_d) for bf16 calls, 2^-21 for the two parts of fp32 calls. The largest stands at 2^5 or more, so
+    those below 2^-19 of it (two parts: 2^-8) have parts under fp16's normal range, off by 2^-25, 2^-30 of the largest;
   * scales as powers of two in the exponent (bf16, many queries): logarithms up to 2^8 to 24 bits, a handful of them, 2^-13;
   * the output's own rounding, 2^-8 or 2^-24 of it."""
 import numpy as np
@@ -67,8 +68,10 @@ def attend(cache, block, b, i, h, q, pos, mask=None, sinks=None):
     w = p * s_v
     out, A = w @ V, w @ V.abs()
     d = big * (D * 2.0 ** -23 + 2.0 ** -21) + 2.0 ** -20
-    tol = A * (d + (n / 16 + 64) * 2.0 ** -23 + (2.0 ** -11 + 2.0 ** -13 if bf16 else 2.0 ** -21)) + out.abs() * (
-        d + (2.0 ** -8 if bf16 else 2.0 ** -23)) + 127 * w.max() * n * 2.0 ** -30
+    alone = min(n, 128 * (k.shape[0] * k.shape[1] * -(-k.shape[2] // 128) / 148 + 2))
+    tiny = int((w < w.max() * 2.0 ** (-19 if bf16 else -8)).sum())
+    tol = A * (d + (alone / 16 + 128) * 2.0 ** -23 + (2.0 ** -11 + 2.0 ** -13 if bf16 else 2.0 ** -21)) + out.abs() * (
+        d + (2.0 ** -8 if bf16 else 2.0 ** -23)) + 127 * w.max() * tiny * 2.0 ** -30
     return out, tol
 
 
@@ -133,6 +136,53 @@ def test_blocks_of_tiny_values_count_in_the_sum(T, D, tiny):
     c = KVCache8.from_tensors(*cache, block)
     y = c.attn(q, i32([S - T]))
     check(y, cache, block, some_queries(1, T, H * rep), q, [S - T])
+    assert status() == 0
+
+
+FAR = [(T, D, dtype) for T, dtype in ((1, "bf16"), (1, "fp32"), (5, "bf16"), (5, "fp32")) for D in (64, 128, 256)]
+
+
+def hidden_case(T, D, dtype, r):
+    """Blocks of values times r that a mask hides from all queries, the first of all among them."""
+    H, rep, S, block = 2, 4, 120000 if T <= 5 else 38000, 32
+    cache = rand_cache(T + D, 1, H, S, D, block)
+    hide = torch.arange(cache[3].shape[2], device="cuda") * 7919 % 11 == 0
+    cache[3][:, :, hide] *= r
+    mask = torch.zeros(1, 1, S, device="cuda").masked_fill_(hide.repeat_interleave(block)[:S], -np.inf)
+    q = rand_q(T, (1, T, H * rep, D), dtype)
+    y = KVCache8.from_tensors(*cache, block).attn(q, i32([S - T]), mask=mask)
+    check(y, cache, block, some_queries(1, T, H * rep), q, [S - T], mask)
+
+
+def later_case(T, D, dtype, r):
+    """The last token's values, in a block of their own, times r: the tokens before it do not see them."""
+    H, rep, S, block = 2, 2 if T <= 5 else 4, 113, 16         # a tile of 10, 80 or 240 queries
+    cache = rand_cache(T + D, 2, H, S, D, block)
+    cache[3][:, :, -1] *= r
+    q = rand_q(T, (2, T, H * rep, D), dtype)
+    y = KVCache8.from_tensors(*cache, block).attn(q, i32([S - T, S - T]))
+    check(y, cache, block, some_queries(2, T, H * rep, 12), q, [S - T, S - T])
+
+
+def light_case(T, D, dtype, r):
+    """Blocks of values times r at low scores: they weigh what e^x r makes of them, next to nothing or nearly all."""
+    H, rep, S, block = 2, 4, 120000 if T <= 5 else 38000, 32
+    cache = rand_cache(T + D, 1, H, S, D, block)
+    light = torch.arange(cache[3].shape[2], device="cuda") * 7919 % 11 == 0
+    cache[3][:, :, light] *= r
+    cache[0][:, :, light.repeat_interleave(block)[:S]] = -127
+    q = rand_q(T, (1, T, H * rep, D), dtype).abs()
+    y = KVCache8.from_tensors(*cache, block).attn(q, i32([S - T]))
+    check(y, cache, block, some_queries(1, T, H * rep), q, [S - T])
+
+
+@pytest.mark.parametrize("r", [1e4, 1e8, 1e30])
+@pytest.mark.parametrize("case", [hidden_case, later_case, light_case])
+@pytest.mark.parametrize("T,D,dtype", FAR)
+def test_value_scales_far_apart(T, D, dtype, case, r):
+    if case is later_case and T == 1:
+        pytest.skip("one token: none before it")
+    case(T, D, dtype, r)
     assert status() == 0
 
 
