@@ -3,10 +3,11 @@
 // 128 queries x 128 rows:
 //   S = Q . K^T      tcgen05 kind::f16, Q and the decoded codes of K from shared memory, S in tensor memory
 //   O += P . V       P (fp16, written over S) from tensor memory, the decoded codes of V from shared memory
-// The codes become fp16 exactly (|c| <= 127); K's scales multiply the finished scores, V's the weights, as in the
-// kernel for few queries, and so its choices: weights w = 2^(x - m) s_v c as fp16, m raised
-// only when a score passes it by 2^6 (e^4 with a mask, scores then in natural units). q is fp16 scaled by a power of two
-// to [256, 512): exact but for values 2^-22 below the row's largest.
+// The codes become fp16 exactly (|c| <= 127). K's scales multiply the finished scores, whose reference m is raised only when
+// one passes it by 2^6 (e^4 with a mask, scores then in natural units). V's scales go into the weights' exponents,
+//   w = 2^(x - m + log2 s_v - d + 8)  as fp16 (2^-11 of it; 2^-33 of the query's largest where it is tiny beside that one),
+// d the query's own, raised when a weight passes it by 2^6: only rows that the query sees set it, by what they weigh.
+// q is fp16 scaled by a power of two to [256, 512): exact but for values 2^-22 below the row's largest.
 //
 // One CTA per SM walks its part of the list of units (128 rows of one tile and kv head; Walk). Warp roles:
 //  * softmax warps, eight per query tile: a thread is a query and one half of a row tile's columns, so that the time
@@ -19,7 +20,7 @@
 // QT = 2 query tiles share a decoded row tile and alternate: one's softmax runs beside the other's products. QT = 1
 // (at most 128 queries) alternates two S buffers instead.
 //
-// Measured: 512 tokens over 16.8k rows, 40 query heads on 8 kv heads of 128: 255 to 261 us (0.41 of the products' floor at the
+// Measured: 512 tokens over 16.8k rows, 40 query heads on 8 kv heads of 128: 253 to 258 us (0.41 of the products' floor at the
 // measured bf16 rate; 1088 us in the kernel for few queries). With the work of a role left out, the same call takes 118 us
 // without any, 185 with the products alone, 209 with the decoding too: what is left besides the products is the chain from
 // one role to the next, several times per 128 rows, and the softmax's part of it. 128 columns a softmax thread: 280 to 298;
@@ -44,6 +45,7 @@ namespace {
 constexpr int kRows = 128;                               // rows of a tile, queries of a tile
 constexpr int kSub = kRows * 128;                        // bytes of 128 rows x 64 fp16
 constexpr int kBars = 24;
+constexpr float kTop = 8.f;                              // log2 of the weight that a query's largest begins as (fp16 holds 2^15)
 constexpr int kDec = 3;                                  // decode warps: 12 or 20 warps in all, 3 or 5 a scheduler
 
 template <int DP, int QT>
@@ -217,7 +219,8 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
             const int edge = __shfl_sync(0xffffffffu, lim, 0) + 1;   // lane 0's is the warp's smallest, or -1: nothing valid
             const float *mrow = MASK ? p.mask + b * p.mbs + tok * p.mts : nullptr;
 
-            float m = 0.f, l = 0.f, cv = 0.f;
+            // m: the scores' reference; d: the weights', above m's and in log2 units: w = 2^((x - m) U + log2(s_v) - d + kTop)
+            float m = 0.f, l = 0.f, d = -INFINITY;
             bool have = false;                                   // m is a score's
             for (int j = 0; j < n; ++j) {
                 const int r0 = row0 + j * kRows, buf = QT == 2 ? qt : ns & 1;
@@ -225,11 +228,8 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                 const float scj = sc;
                 if (j + 1 < n) sc = load_scale(r0 + kRows);
                 const bool live = edge > 0;                      // a warp without a valid query leaves its lanes of P as they are
-                // V's largest scale (bits: NaN does not count) against the weights' power of two
-                uint32_t vb = lane >= 8 && lane < 16 ? __float_as_uint(scj) : 0u;
-                vb = __reduce_max_sync(0xffffffffu, vb <= 0x7f800000u ? vb : 0u);
-                const float vmax = __uint_as_float(vb);
-                // O times a, once its last product is done: this half of its columns
+                // O times a, once its last product is done: this half of its columns (at most once a tile: the stores are waited for
+                // with the weights')
                 const auto rescale_o = [&](float a) {
                     if (j == 0 || !live) return;                 // O begins with this tile
                     if (!failed) failed = __any_sync(0xffffffffu, !wait_o(pv - 1));
@@ -242,28 +242,19 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                         for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * a);
                         tc_st_32x32b_x16(otm + 16 * ch, v);
                     }
-                    tc_wait_st();                                // a second rescaling of the same tile loads what this one stored
                 };
-                if (vmax * cv > 512.f || (cv == 0.f && vmax > 0.f)) {
-                    const float cn = pow2_to(vmax, 7);
-                    if (cv != 0.f) rescale_o(cn / cv);
-                    cv = cn;
-                }
-                // what the four 16-column groups of this half need: K's scale with the query's, V's with the power of two
-                float fk[4], wv[4], lg[4], rv[4];
+                // what the four 16-column groups of this half need: K's scale with the query's, the logarithm of V's
+                float fk[4], lg[4], topg[4];
                 {
-                    const float vv = cv * scj, lv = __log2f(vv), iv = __frcp_rn(vv);
+                    const float lv = __log2f(scj);
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
                         fk[g] = rs * __shfl_sync(0xffffffffu, scj, 4 * hf + g);
-                        wv[g] = __shfl_sync(0xffffffffu, vv, 8 + 4 * hf + g);
                         lg[g] = __shfl_sync(0xffffffffu, lv, 8 + 4 * hf + g);
-                        rv[g] = __shfl_sync(0xffffffffu, iv, 8 + 4 * hf + g);
+                        topg[g] = -INFINITY;
                     }
                 }
-                // (where V's scales are far apart, s_v c and the weights with it would underflow and be missing in the sum)
-                const bool near = !(lane >= 8 && lane < 16 && !(cv * scj > 0x1p-40f));
-                const bool usual = !MASK && r0 + kRows <= edge && __all_sync(0xffffffffu, near);
+                const bool clear = !MASK && r0 + kRows <= edge;  // every query of the warp sees every row
                 const uint32_t sphase = QT == 2 ? ns & 1 : ns >> 1 & 1;
                 if (!failed) failed = __any_sync(0xffffffffu, !mbar_wait_bounded(s_full + 8 * buf, sphase, kWaitNs));
                 ++ns;
@@ -277,8 +268,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                     }
                     return col <= lim ? x : -INFINITY;
                 };
-                // the largest score of this half
-                float top = -INFINITY;
+                // the largest scores of this half's groups
                 if (live) {
 #pragma unroll
                     for (int ch = 0; ch < 2; ++ch) {
@@ -288,7 +278,7 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
                             const float f = fk[2 * ch + g];
-                            if (usual) {                         // scales are not negative
+                            if (clear) {                         // scales are not negative
                                 float t0 = __uint_as_float(s[16 * g]), t1 = __uint_as_float(s[16 * g + 1]);
 #pragma unroll
                                 for (int k = 2; k < 14; k += 4) {
@@ -296,27 +286,55 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                                     t1 = max3(t1, __uint_as_float(s[16 * g + k + 2]), __uint_as_float(s[16 * g + k + 3]));
                                 }
                                 t0 = max3(t0, __uint_as_float(s[16 * g + 14]), __uint_as_float(s[16 * g + 15]));
-                                top = fmaxf(top, fmaxf(t0, t1) * f);
+                                topg[2 * ch + g] = fmaxf(-INFINITY, fmaxf(t0, t1) * f);      // NaN is none
                             } else {
+                                float t = -INFINITY;
 #pragma unroll
-                                for (int k = 0; k < 16; ++k) top = fmaxf(top, score(s[16 * g + k], f, r0 + 64 * hf + 32 * ch + 16 * g + k));
+                                for (int k = 0; k < 16; ++k) t = fmaxf(t, score(s[16 * g + k], f, r0 + 64 * hf + 32 * ch + 16 * g + k));
+                                topg[2 * ch + g] = t;
                             }
                         }
                     }
                 }
-                if (bar_any(2 + qt, 256, top > m + RAISE || (!have && top > -INFINITY))) {
+                float top = fmaxf(fmaxf(topg[0], topg[1]), fmaxf(topg[2], topg[3]));
+                // the largest weight, relative to m
+                const auto heaviest = [&] {
+                    float y = -INFINITY;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) y = fmaxf(y, fmaf(topg[g] - m, U, lg[g]));
+                    return y;
+                };
+                if (bar_any(2 + qt, 256, have ? top > m + RAISE || heaviest() > d + 6.f : top > -INFINITY)) {
                     *mine = top;
                     named_bar_sync(2 + qt, 256);
                     top = fmaxf(top, *other);                    // the row's, in both its threads
-                    float a = 1.f;
-                    if (top > m + RAISE || (!have && top > -INFINITY)) {
-                        a = have ? ex2((m - top) * U) : 0.f;
+                    if (have ? top > m : top > -INFINITY) {      // the weights so far stay what they are: d falls as m rises
+                        const float by = have ? (m - top) * U : 0.f;
+                        l *= ex2(by);
+                        d += by;
                         m = top;
-                        l *= a;
                         have = true;
+                    }
+                    named_bar_sync(2 + qt, 256);
+                    float y = heaviest();
+                    *mine = y;
+                    named_bar_sync(2 + qt, 256);
+                    y = fmaxf(y, *other);
+                    float a = 1.f;
+                    if (y > d + 6.f) {
+                        a = ex2(d - y);
+                        d = y;
                     }
                     if (__any_sync(0xffffffffu, a != 1.f)) rescale_o(a);
                 }
+                float sh[4];                                     // a group's log2(s_v) - d + kTop
+                bool near = true;                                // and weights that do not underflow in the sum
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    sh[g] = lg[g] - (d == -INFINITY ? 0.f : d) + kTop;
+                    near &= sh[g] > -80.f;
+                }
+                const bool usual = clear && __all_sync(0xffffffffu, near);
                 // the weights of this half
                 if (live) {
 #pragma unroll
@@ -329,9 +347,9 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                             const float f = fk[2 * ch + g];
                             float s0 = 0.f, s1 = 0.f;
                             if (usual) {
-                                // V's scales are above 0 and alike: a weight is one exponential, w = 2^(S f - m + log2(s_v c)), and the
-                                // sum takes w / (s_v c)
-                                const float at = lg[2 * ch + g] - m;
+                                // V's scales are above 0 and none is far below d: a weight is one exponential, and the sum
+                                // takes it times 2^-sh
+                                const float at = sh[2 * ch + g] - m;
 #pragma unroll
                                 for (int k = 0; k < 16; k += 2) {
                                     const float w0 = ex2(fmaf(__uint_as_float(s[16 * g + k]), f, at));
@@ -340,18 +358,18 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                                     s1 += w1;
                                     ph[8 * g + k / 2] = pack_h2(w0, w1);
                                 }
-                                l = fmaf(s0 + s1, rv[2 * ch + g], l);
+                                l = fmaf(s0 + s1, ex2(-sh[2 * ch + g]), l);
                             } else {
-                                const float wg = wv[2 * ch + g];
+                                const float at = sh[2 * ch + g];
                                 const int col = r0 + 64 * hf + 32 * ch + 16 * g;
 #pragma unroll
                                 for (int k = 0; k < 16; k += 2) {
                                     const float x0 = score(s[16 * g + k], f, col + k), x1 = score(s[16 * g + k + 1], f, col + k + 1);
-                                    const float e0 = ex2((x0 - m) * U), e1 = ex2((x1 - m) * U);
-                                    s0 += e0;
-                                    s1 += e1;
+                                    s0 += ex2((x0 - m) * U);
+                                    s1 += ex2((x1 - m) * U);
                                     // a row that is not seen weighs nothing, even where its scale is NaN
-                                    ph[8 * g + k / 2] = pack_h2(x0 == -INFINITY ? 0.f : e0 * wg, x1 == -INFINITY ? 0.f : e1 * wg);
+                                    ph[8 * g + k / 2] = pack_h2(x0 == -INFINITY ? 0.f : ex2(fmaf(x0 - m, U, at)),
+                                                                x1 == -INFINITY ? 0.f : ex2(fmaf(x1 - m, U, at)));
                                 }
                                 l += s0 + s1;
                             }
@@ -371,10 +389,11 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
             *mine = l;
             named_bar_sync(2 + qt, 256);
             l += *other;                                         // the sum of both halves
-            // O c^-1 relative to m: the output, or a partial; each half of the threads its half of the columns
-            const float M = have ? m : -INFINITY, inv = cv == 0.f ? 1.f : 1.f / cv;
-            float so, f = inv;
-            if (wk.whole()) f = out_factor<MASK>(M, l, p.sinks, hq, so) * so * inv;
+            // O 2^(d - kTop) relative to m: the output, or a partial; each half of the threads its half of the columns. The factor
+            // by halves, d may pass fp32's exponents
+            const float M = have ? m : -INFINITY, half = ex2(0.5f * ((d == -INFINITY ? 0.f : d) - kTop));
+            float so, f = half;
+            if (wk.whole()) f = out_factor<MASK>(M, l, p.sinks, hq, so) * so * half;
             const int64_t oo = (static_cast<int64_t>(b) * p.r.T + tok) * p.ldo + static_cast<int64_t>(hq) * D;
             float *po = slot_o<DP>(p.ws, QT * kRows, wk.slot(blockIdx.x)) + static_cast<int64_t>(qi) * DP;
 #pragma unroll 1
@@ -387,8 +406,8 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
 #pragma unroll
                 for (int k = 0; k < 32; k += 4) {
                     const int d = 32 * ch + k;
-                    const float4 y = make_float4(__uint_as_float(v[k]) * f, __uint_as_float(v[k + 1]) * f,
-                                                 __uint_as_float(v[k + 2]) * f, __uint_as_float(v[k + 3]) * f);
+                    const float4 y = make_float4(__uint_as_float(v[k]) * half * f, __uint_as_float(v[k + 1]) * half * f,
+                                                 __uint_as_float(v[k + 2]) * half * f, __uint_as_float(v[k + 3]) * half * f);
                     if (d < D) {
                         if (wk.whole()) store4<true>(p.out, oo + d, y);
                         else *reinterpret_cast<float4 *>(po + d) = y;

@@ -139,7 +139,8 @@ def test_blocks_of_tiny_values_count_in_the_sum(T, D, tiny):
     assert status() == 0
 
 
-FAR = [(T, D, dtype) for T, dtype in ((1, "bf16"), (1, "fp32"), (5, "bf16"), (5, "fp32")) for D in (64, 128, 256)]
+FAR = [(T, D, dtype) for T, dtype in ((1, "bf16"), (1, "fp32"), (5, "bf16"), (5, "fp32")) for D in (64, 128, 256)] + \
+    [(T, D, "bf16") for T in (20, 60) for D in (64, 128)]
 
 
 def hidden_case(T, D, dtype, r):
