@@ -6,6 +6,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "kernels.h"
 #include "tmap.h"
@@ -64,6 +65,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {     // NaN where ei
     return d;
 }
 
+// a / b, in 32 bits where they fit (they all but always do; a 64-bit division costs a few hundred instructions)
+__device__ __forceinline__ int64_t div64(int64_t a, int64_t b) {
+    if (((a | b) >> 31) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+
 // ---------------------------------------------------------------- the list of units
 // An entry is a (sequence, query tile); its rows are counted in units of `unit` rows, once per kv head.
 struct Plan {
@@ -83,7 +90,7 @@ struct Plan {
         if (!kv8_rows(p.r, b, p.c.S, pos, cnt)) return 0;
         if (tiles == 1) return cnt > 0 ? pos + cnt : 0;
         const int64_t r0 = static_cast<int64_t>(e - b * tiles) * tile;
-        const int first = static_cast<int>(r0 / rep), last = static_cast<int>((r0 + tile - 1) / rep);
+        const int first = static_cast<int>(div64(r0, rep)), last = static_cast<int>(div64(r0 + tile - 1, rep));
         if (first >= cnt) return 0;
         return pos + min(last, cnt - 1) + 1;
     }
@@ -99,11 +106,6 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
-}
-// a / b, in 32 bits where they fit (they all but always do; a 64-bit division costs a few hundred instructions)
-__device__ __forceinline__ int64_t div64(int64_t a, int64_t b) {
-    if (((a | b) >> 31) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-    return a / b;
 }
 // units a CTA takes: N units over G CTAs; CTA i has units [i * per, (i + 1) * per) of the list. (At least two each: one
 // token over 4096 rows 10.0 us against 10.5, over 77 rows 9.5 against 6.3.)
@@ -219,12 +221,13 @@ struct Walk {
 };
 
 
-// Which CTAs hold entry e's rows for head h, and in which of their slots: a CTA's first segment is in its slot 0, its
+// Which CTAs hold an entry's rows for one head, and in which of their slots: a CTA's first segment is in its slot 0, its
 // last in slot 1. i0 == i1: one has them all.
 struct Shares {
-    int b, cnt, i0, i1, s0;
+    int b, cnt, h, i0, i1, s0;
     int64_t q0;                       // the tile's first query
-    __device__ __forceinline__ Shares(const Kv8AttnParams &p, const Plan &pl, int lane, int e, int h, int G) {
+    // entry e's for head h_; every lane of the warp goes through the list
+    __device__ __forceinline__ Shares(const Kv8AttnParams &p, const Plan &pl, int lane, int e, int h_, int G) {
         int64_t before = 0, all = 0;
         for (int i = lane; i < pl.entries; i += 32) {
             const int v = pl.units(p, i);
@@ -233,15 +236,78 @@ struct Shares {
         }
         int pos;
         const int n = pl.units_of(pl.rows(p, e, pos, cnt));
+        h = h_;
+        tile_of(pl, e);
+        const int64_t N = warp_sum64(all) * p.c.Hkv, u = warp_sum64(before) * p.c.Hkv + static_cast<int64_t>(h) * n;
+        set(u, n, units_per_cta(N, G));
+    }
+    // those that CTA i's last segment is shared with, where it is the first to have a part of it (else none: i0 == i1). A block
+    // of THREADS goes through the list together, a run of entries a thread.
+    template <int THREADS>
+    __device__ __forceinline__ Shares(const Kv8AttnParams &p, const Plan &pl, int i, int G, std::integral_constant<int, THREADS>) {
+        __shared__ int64_t sums[THREADS / 32], at_e0;
+        __shared__ int at_e, at_n;
+        const int t = threadIdx.x, lane = t & 31, run = (pl.entries + THREADS - 1) / THREADS;
+        const int e0 = static_cast<int>(min(static_cast<int64_t>(pl.entries), static_cast<int64_t>(t) * run));
+        const int e1 = static_cast<int>(min(static_cast<int64_t>(pl.entries), static_cast<int64_t>(e0) + run));
+        int64_t mine = 0;
+        for (int e = e0; e < e1; ++e) mine += pl.units(p, e);
+        int64_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += up;
+        }
+        if (lane == 31) sums[t >> 5] = incl;
+        if (t == 0) at_n = 0;
+        __syncthreads();
+        int64_t N = 0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; ++w) {
+            if (w < t >> 5) incl += sums[w];
+            N += sums[w];
+        }
+        N *= p.c.Hkv;
+        const int64_t per = units_per_cta(N, G), border = per * (i + 1);
+        int64_t u = (incl - mine) * p.c.Hkv;
+        if (border >= u && border < incl * p.c.Hkv) {              // one thread's, if any
+            for (int e = e0; e < e1; ++e) {
+                const int n = pl.units(p, e);
+                if (border < u + static_cast<int64_t>(n) * p.c.Hkv) {
+                    at_e = e;
+                    at_n = n;
+                    at_e0 = u;
+                    break;
+                }
+                u += static_cast<int64_t>(n) * p.c.Hkv;
+            }
+        }
+        __syncthreads();
+        b = cnt = h = i0 = i1 = s0 = 0;
+        q0 = 0;
+        const int n = at_n;
+        if (n == 0) return;                                        // the list ends before the border
+        h = static_cast<int>(div64(border - at_e0, n));
+        u = at_e0 + static_cast<int64_t>(h) * n;
+        if (u == border) return;                                   // a segment begins there
+        set(u, n, per);
+        if (i0 != i) i1 = i0;                                      // an earlier border's
+        int pos;
+        pl.rows(p, at_e, pos, cnt);
+        tile_of(pl, at_e);
+    }
+    __device__ __forceinline__ int slot(int i) const { return i == i0 ? s0 : 2 * i; }
+
+private:
+    __device__ __forceinline__ void tile_of(const Plan &pl, int e) {
         b = pl.tiles == 1 ? e : e / pl.tiles;
         q0 = static_cast<int64_t>(e - b * pl.tiles) * pl.tile;
-        const int64_t N = warp_sum64(all) * p.c.Hkv, u = warp_sum64(before) * p.c.Hkv + static_cast<int64_t>(h) * n;
-        const int64_t per = units_per_cta(N, G);
+    }
+    __device__ __forceinline__ void set(int64_t u, int n, int64_t per) {
         i0 = n ? static_cast<int>(div64(u, per)) : 0;
         i1 = n ? static_cast<int>(div64(u + n - 1, per)) : 0;
         s0 = 2 * i0 + (i0 * per < u ? 1 : 0);
     }
-    __device__ __forceinline__ int slot(int i) const { return i == i0 ? s0 : 2 * i; }
 };
 
 template <bool BF16>

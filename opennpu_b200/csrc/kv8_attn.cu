@@ -603,17 +603,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_kernel(const Kv
 }
 
 // The same where a segment has few parts: up to kJoinRows queries of a tile a CTA, a warp at a time on each of its
-// share (a CTA for each query took 161 us of a 512-token chunk's 450).
+// share (a CTA for each query took 161 us of a 512-token chunk's 450). Of more segments than the split kernel has CTAs at most
+// one is shared over each border between two of them, so CTAs are for borders then: many short sequences or query tiles have few
+// partials, and a CTA for each segment, each with its way through the list, took 1240 of 1282 us at 4096 sequences.
 constexpr int kJoinRows = 32;
 
-template <int DP, bool BF16, bool MASK>
+template <int DP, bool BF16, bool MASK, bool BORDERS>
 __global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_rows_kernel(const Kv8AttnParams p, int G, int tile, int unit) {
     constexpr float U = MASK ? kLog2e : 1.f;
     constexpr int V = DP == 256 ? 2 : 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.c.D, rows = min(tile, kJoinRows), groups = tile / rows;
     const Plan pl(p, tile, unit);
-    const int eh = blockIdx.x / groups, qg = (blockIdx.x - eh * groups) * rows, e = eh / p.c.Hkv, h = eh - e * p.c.Hkv;
-    const Shares sh(p, pl, lane, e, h, G);
+    const int at = blockIdx.x / groups, qg = (blockIdx.x - at * groups) * rows;
+    const Shares sh = [&] {
+        if constexpr (BORDERS) return Shares(p, pl, at, G, std::integral_constant<int, kJoinWarps * 32>{});
+        else return Shares(p, pl, lane, at / p.c.Hkv, at % p.c.Hkv, G);
+    }();
+    const int h = sh.h;
     pdl_wait_prerequisites();
     pdl_launch_dependents();
     if (sh.i0 == sh.i1) return;                                // one CTA had it all and wrote the outputs
@@ -683,11 +689,14 @@ cudaError_t join_launch(const Kv8AttnParams &p, int G, int tile, int unit, cudaS
     // one query's. One token of 64 sequences (256 segments): 51.9 us by rows, 58.1 by queries; one sequence of 131001 rows
     // (8 segments, 55 parts each): 56.8 by rows, 49.4 by queries.
     const int64_t segments = tiles * p.c.B * p.c.Hkv;
-    const bool by_rows = segments * 4 >= G;
-    const int64_t joins = segments * (by_rows ? tile / std::min(tile, kJoinRows) : tile);
-    if (joins > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    return launch_pdl(by_rows ? kv8_attn_join_rows_kernel<DP, BF16, MASK> : kv8_attn_join_kernel<DP, BF16, MASK>,
-                      dim3(static_cast<unsigned>(joins)), dim3(kJoinWarps * 32), 0, s, p, G, tile, unit);
+    const bool by_rows = segments * 4 >= G, borders = segments > G - 1;
+    const int64_t joins = borders ? static_cast<int64_t>(G - 1) * (tile / std::min(tile, kJoinRows))
+                                  : segments * (by_rows ? tile / std::min(tile, kJoinRows) : tile);
+    if (joins == 0) return cudaSuccess;
+    const auto k = borders   ? kv8_attn_join_rows_kernel<DP, BF16, MASK, true>
+                   : by_rows ? kv8_attn_join_rows_kernel<DP, BF16, MASK, false>
+                             : kv8_attn_join_kernel<DP, BF16, MASK>;
+    return launch_pdl(k, dim3(static_cast<unsigned>(joins)), dim3(kJoinWarps * 32), 0, s, p, G, tile, unit);
 }
 
 template <int DP, int NT, bool BF16, bool MASK>

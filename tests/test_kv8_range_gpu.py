@@ -187,6 +187,30 @@ def test_value_scales_far_apart(T, D, dtype, case, r):
     assert status() == 0
 
 
+# ---------------------------------------------------------------- more sequences and tiles than CTAs
+@pytest.mark.parametrize("B,T,Hq,H,D,S,dtype,long", [
+    (3000, 1, 8, 2, 64, 90, "bf16", 0), (700, 2, 16, 4, 128, 64, "fp32", 0), (150, 1, 8, 4, 256, 3000, "bf16", 70),
+    (600, 1, 16, 2, 128, 5000, "fp32", 9), (1, 700, 4, 2, 256, 1500, "bf16", 0), (3, 300, 8, 2, 64, 900, "fp32", 0),
+    (90, 20, 8, 2, 64, 1500, "bf16", 30), (40, 33, 16, 2, 128, 2500, "bf16", 11), (5, 500, 16, 4, 128, 700, "bf16", 0)])
+def test_many_sequences_and_query_tiles(B, T, Hq, H, D, S, dtype, long):
+    """More (sequence, query tile, head) segments than CTAs, of mixed lengths, some sequences without tokens: parts of a segment
+    are joined where a border between two CTAs falls into it. Every `long`-th sequence is full, the others short."""
+    block = 32
+    cache = rand_cache(B, B, H, S, D, block)
+    rng = np.random.default_rng(B + T)
+    end = np.where(np.arange(B) % long == 0, S, rng.integers(T, T + 60, B)) if long else rng.integers(T, S + 1, B)
+    cnt = np.where(rng.random(B) < (0.1 if B > 9 else 0), 0, T)
+    cnt[[0, -1]] = T
+    pos = end - T
+    q = rand_q(B, (B, T, Hq, D), dtype)
+    out = torch.full_like(q, 7)
+    KVCache8.from_tensors(*cache, block).attn(q, i32(pos), i32(cnt), out=out)
+    check(out, cache, block, [c for c in some_queries(B, T, Hq, 60) if cnt[c[0]]], q, pos)
+    idle = torch.from_numpy(cnt == 0)
+    assert (out[idle.cuda()] == 7).all() and torch.isfinite(out).all() and not (out[~idle.cuda()] == 7).all(-1).any()
+    assert status() == 0
+
+
 # ---------------------------------------------------------------- calls of several threads
 FIRST_CALLS_AT_ONCE = """
 import threading
