@@ -314,9 +314,9 @@ cudaError_t kv8_read_launch(const Kv8Cache &c, const Kv8Rows &r, void *k, int64_
                             bool bf16, cudaStream_t stream) {
     const Kv8Out out{{k, v}, {ldk, ldv}};
     // a CTA's rows: at least one vector for each of its threads, at most four rounds of kReadFly; in between
-    // as many as leave eight CTAs for each of the 148 SMs
+    // as many as leave eight CTAs for each SM
     const int64_t one = std::max<int64_t>(1, kReadThreads / (static_cast<int64_t>(c.Hkv) * c.D / 8));
-    const int64_t spread = static_cast<int64_t>(r.T) * 2 * c.B / (8 * 148);
+    const int64_t spread = static_cast<int64_t>(r.T) * 2 * c.B / (8 * std::max(1, kv8_sms()));
     const int rows = static_cast<int>(std::min(std::max(one, spread), 4 * kReadFly * one));
     const dim3 grid((r.T - 1) / rows + 1, 2 * c.B);
     return bf16 ? launch_pdl(kv8_read_kernel<true>, grid, dim3(kReadThreads), 0, stream, c, r, out, rows, RowDiv(c.D))

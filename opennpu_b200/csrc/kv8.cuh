@@ -4,6 +4,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <type_traits>
@@ -335,15 +336,28 @@ __device__ __forceinline__ float out_factor(float M, float Lsum, const float *si
     return total == 0.f ? 0.f : 1.f / total;
 }
 
-// (host) SMs of the current device
-inline int kv8_sms() {
-    static const int n = [] {
-        int dev = 0, v = 0;
-        cudaGetDevice(&dev);
-        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
-        return v > 0 ? v : 1;
-    }();
+// (host) f()'s value where it is above 0 (kept from then on), else what a lookup that failed gave: asked for again at the next call
+template <typename F>
+int kv8_kept(std::atomic<int> &kept, F f) {
+    int n = kept.load(std::memory_order_relaxed);
+    if (n <= 0) {
+        n = f();
+        if (n > 0) kept.store(n, std::memory_order_relaxed);
+    }
     return n;
+}
+// (host) the error of such a lookup
+inline cudaError_t kv8_lookup_error() {
+    const cudaError_t e = cudaGetLastError();
+    return e != cudaSuccess ? e : cudaErrorInvalidConfiguration;
+}
+// (host) SMs of the current device; 0: the lookup failed
+inline int kv8_sms() {
+    static std::atomic<int> kept{0};
+    return kv8_kept(kept, [] {
+        int dev = 0, v = 0;
+        return cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess ? v : 0;
+    });
 }
 // (host) a map of [batch][heads][rows][dim] codes whose boxes are `rows` rows of at most 128 codes, their 16-byte
 // chunks exchanged by `swizzle`; columns and rows past the ends read 0

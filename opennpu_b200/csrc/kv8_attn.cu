@@ -705,19 +705,20 @@ struct Split {
     static constexpr int R = DP == 256 ? 1 : 2, NS = R == 1 ? 3 : 2;
     static constexpr int ring = kWarps * NS * kStageBytes<DP, R>, merge = kMergeBytes<DP, NT>;
     static constexpr int smem = 1024 + (ring > merge ? ring : merge);
-    static int ctas() {                                        // one resident wave
-        static const int n = [] {
+    static int ctas() {                                        // one resident wave; 0: the lookup failed
+        static std::atomic<int> kept{0};
+        return kv8_kept(kept, [] {
             auto k = kv8_attn_split_kernel<DP, NT, BF16, MASK, R, NS>;
             int per = 0;
             if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-                cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, k, kWarps * 32, smem) != cudaSuccess || per < 1)
-                per = 1;
+                cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, k, kWarps * 32, smem) != cudaSuccess)
+                return 0;
             return per * kv8_sms();
-        }();
-        return n;
+        });
     }
     static cudaError_t launch(const Kv8AttnParams &p, cudaStream_t s) {
         const int G = ctas(), rep = p.Hq / p.c.Hkv;
+        if (G < 1) return kv8_lookup_error();
         const int64_t tiles = (static_cast<int64_t>(p.r.T) * rep + 8 * NT - 1) / (8 * NT);
         if (tiles * p.c.B > 0x7fffffff) return cudaErrorInvalidConfiguration;
         CUtensorMap mk, mv;
@@ -761,9 +762,11 @@ int64_t kv8_attn_ws_bytes(int Hq, int Hkv, int D, int T, bool bf16) {
     if (use_tiles(D, queries, bf16)) {
         G = kv8_tile_ctas();
         tile = kv8_tile_queries(queries);
+        if (G < 1) return -1;
     } else {
         for (const bool mask : {false, true}) {
             const int64_t g = with_split(D, queries, bf16, mask, [](auto k) { return static_cast<int64_t>(k.ctas()); });
+            if (g < 1) return -1;
             G = g > G ? g : G;
         }
     }
@@ -775,6 +778,7 @@ cudaError_t kv8_attn_launch(const Kv8AttnParams &p, bool bf16, cudaStream_t s) {
     if (!use_tiles(p.c.D, queries, bf16))
         return with_split(p.c.D, queries, bf16, p.mask != nullptr, [&](auto k) { return k.launch(p, s); });
     const int G = kv8_tile_ctas(), tile = kv8_tile_queries(queries), unit = kv8_tile_rows();
+    if (G < 1) return kv8_lookup_error();
     if ((queries + tile - 1) / tile * p.c.B > 0x7fffffff) return cudaErrorInvalidConfiguration;
     const cudaError_t e = kv8_tile_launch(p, s);
     if (e != cudaSuccess) return e;

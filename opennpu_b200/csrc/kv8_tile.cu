@@ -529,8 +529,9 @@ template <int DP, int QT, bool MASK>
 cudaError_t launch_t(const Kv8AttnParams &p, cudaStream_t s) {
     using Z = TileSizes<DP, QT>;
     const auto k = kv8_attn_tile_kernel<DP, QT, MASK>;
-    static const cudaError_t attr = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::smem);
-    if (attr != cudaSuccess) return attr;
+    static std::atomic<int> kept{0};
+    if (!kv8_kept(kept, [&] { return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::smem) == cudaSuccess ? 1 : 0; }))
+        return kv8_lookup_error();
     CUtensorMap mk, mv;
     if (!kv8_code_map(mk, p.c, p.c.k, DP, kRows, CU_TENSOR_MAP_SWIZZLE_NONE) ||
         !kv8_code_map(mv, p.c, p.c.v, DP, kRows, CU_TENSOR_MAP_SWIZZLE_NONE))

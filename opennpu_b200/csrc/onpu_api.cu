@@ -2863,7 +2863,9 @@ int64_t onpu_kv8_attn_ws(const onpu_kv8_cache *cache, int Hq, int64_t T, int x_b
     if (!kv8_check(who, cache, T, &none, nullptr, c, r) || !kv8_check_heads(who, cache, Hq) ||
         !kv8_device(who, r))
         return -1;
-    return kv8_attn_ws_bytes(Hq, c.Hkv, c.D, r.T, x_bf16 != 0);
+    const int64_t n = kv8_attn_ws_bytes(Hq, c.Hkv, c.D, r.T, x_bf16 != 0);
+    if (n < 0) set_err("%s: looking up the kernels failed: %s", who, cudaGetErrorString(cudaGetLastError()));
+    return n;
 }
 
 int onpu_kv8_attn_dev(const onpu_kv8_cache *cache, const void *q, int64_t ldq, int Hq, int64_t T, int x_bf16,
