@@ -409,12 +409,11 @@ typedef struct onpu_kv8_cache {
  * grow; cnt NULL: T everywhere; cnt[b] = 0 leaves sequence b alone. Token rows (k, v, q, out) lie at
  * (b * T + i) * ld, heads one after another in a row; rows i >= cnt[b] of a padded batch are neither
  * read nor written. They are bf16 (x_bf16 != 0) or fp32, 16-byte aligned, ld times the element a
- * multiple of 16 bytes; pos, cnt, mask and sinks are 4-byte aligned. dim is a multiple of 16, at most 256; batch at
- * most 32767. A sequence whose rows are
- * not all inside the cache, or whose cnt is not in [0, T], is skipped and sets the device status
- * (onpu_check_device). Asynchronous on `stream`, no allocation, capturable; calls that touch the same
- * sequence's rows are ordered by the caller, and pos and cnt stay as they are until a call is done. The device that is current must be the library's.
- * 0 ok, < 0 error.
+ * multiple of 16 bytes; pos, cnt, mask and sinks are 4-byte aligned. dim is a multiple of 16, at most 256; rows at most
+ * 2^31 - 4096, batch at most 32767. A sequence whose rows are not all inside the cache, or whose cnt is not in [0, T], is
+ * skipped and sets the device status (onpu_check_device). Asynchronous on `stream`, no allocation, capturable; calls that
+ * touch the same sequence's rows are ordered by the caller, and pos and cnt stay as they are until a call is done. The device
+ * that is current must be the library's. 0 ok, < 0 error.
  *
  * append: quantises rows k, v [batch * T][heads * dim] into the cache. For each block that holds one
  * of a sequence's new rows: scale = max(old scale, largest |value| of its new rows / 127), the old scale

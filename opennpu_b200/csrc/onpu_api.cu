@@ -2751,9 +2751,9 @@ bool kv8_check(const char *who, const onpu_kv8_cache *d, int64_t T, const int32_
         set_err("%s: pos and cnt must be 4-byte aligned", who);
         return false;
     }
-    if (d->batch < 1 || d->batch > 32767 || d->heads < 1 || d->heads > 65535 || d->rows < 1 || d->rows > 0x7fffff00 ||
+    if (d->batch < 1 || d->batch > 32767 || d->heads < 1 || d->heads > 65535 || d->rows < 1 || d->rows > 0x7ffff000 ||
         d->dim < 16 || d->dim > 256 || d->dim % 16 || (d->block != 16 && d->block != 32 && d->block != 64)) {
-        set_err("%s: need 1 <= batch <= 32767, 1 <= heads <= 65535, 1 <= rows <= 2^31 - 256, dim a multiple of 16 up to "
+        set_err("%s: need 1 <= batch <= 32767, 1 <= heads <= 65535, 1 <= rows <= 2^31 - 4096, dim a multiple of 16 up to "
                 "256, block 16, 32 or 64 (got %lld, %lld, %lld, %lld, %d)", who, static_cast<long long>(d->batch),
                 static_cast<long long>(d->heads), static_cast<long long>(d->rows), static_cast<long long>(d->dim),
                 d->block);

@@ -27,6 +27,16 @@ def test_words_that_are_not_4_byte_aligned_are_refused(fn, bad):
     assert f"onpu_kv8_{fn}_dev" in L.last_error() and "4-byte aligned" in L.last_error()
 
 
+@pytest.mark.parametrize("fn", ["append", "read", "attn"])
+def test_rows_whose_counts_pass_32_bits_are_refused(fn, monkeypatch):
+    """The kernels step up to 2100 rows past a sequence's last in 32 bits."""
+    rows = (1 << 31) - 4095
+    monkeypatch.setattr(DESC, "rows", rows)
+    for name, stride in (("hs", rows * 64), ("bs", 4 * rows * 64), ("shs", 1 << 26), ("sbs", 1 << 28)):
+        monkeypatch.setattr(DESC, name, stride)
+    assert call(fn) < 0 and "2^31 - 4096" in L.last_error()
+
+
 class FakeCuda:
     """What the wrapper looks at of a dense CUDA tensor on device 1."""
     is_cuda, device = True, torch.device("cuda", 1)
