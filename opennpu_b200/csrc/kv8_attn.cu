@@ -675,8 +675,11 @@ int pick_nt(int DP, int64_t queries) {
 }
 // More queries a kv head than this go to 128-query tiles (kv8_tile.cu), where heads fit them and they are bf16 (the tiles'
 // sums over rows stay in the tensor core, which cuts them off: 7.4e-6 off after 16k rows, too much for fp32). us, tiles / this kernel,
-// at 40, 64, 96, 128 queries (bf16, D 128): 8 sequences of about 2250 rows 43 / 59, 45 / 70, 48 / 117, 51 / 146; one
-// sequence of 16000 rows 53 / 33, 55 / 38, 58 / 53, 62 / 66.
+// at 40, 72, 96, 128 queries (bf16, 8 heads of 128): one sequence of 700 rows 16 / 13, 18 / 16, 19 / 18, 21 / 19, of 16000 rows
+// 34 / 33, 36 / 43, 39 / 53, 43 / 66; 8 sequences of 2250 rows 39 / 36, 41 / 53, 43 / 60, 46 / 76. Of 2 heads: one sequence of
+// 700 rows 12 / 11, 13 / 11, 15 / 11, 16 / 12, of 16000 rows 24 / 22, 26 / 20, 28 / 26, 31 / 28, of 64000 rows 33 / 35, 35 / 44, 37 / 49,
+// 40 / 60. What decides is the rows of all sequences and heads, which the host does not know; the few microseconds that
+// short calls lose are less than what long ones would.
 constexpr int kTileFrom = 64;
 bool use_tiles(int D, int64_t queries, bool bf16) { return bf16 && D <= 128 && queries > kTileFrom; }
 int padded_dim(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }

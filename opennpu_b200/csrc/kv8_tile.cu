@@ -12,7 +12,7 @@
 // One CTA per SM walks its part of the list of units (128 rows of one tile and kv head; Walk). Warp roles:
 //  * softmax warps, eight per query tile: a thread is a query and one half of a row tile's columns, so that the time
 //    from scores to weights, which the products wait for, is half as long. Per row tile: the largest score (a barrier with
-//    a vote joins the halves; the reference m is raised only if one asks), then the weights, 32 at a time, written over the
+//    a vote joins the halves; m and d are raised only if one asks), then the weights, 32 at a time, written over the
 //    scores just read. At a segment's end O is scaled and stored (or a partial).
 //  * three decode warps: codes that TMA brought (128 rows, K and V in turn, one of each ahead) to fp16 in the
 //    128-byte-swizzled layout, two stages each. K is read K-major, V (rows are K of the product) MN-major.
@@ -20,7 +20,7 @@
 // QT = 2 query tiles share a decoded row tile and alternate: one's softmax runs beside the other's products. QT = 1
 // (at most 128 queries) alternates two S buffers instead.
 //
-// Measured: 512 tokens over 16.8k rows, 40 query heads on 8 kv heads of 128: 253 to 258 us (0.41 of the products' floor at the
+// Measured: 512 tokens over 16.8k rows, 40 query heads on 8 kv heads of 128: 249 to 254 us (0.42 of the products' floor at the
 // measured bf16 rate; 1088 us in the kernel for few queries). With the work of a role left out, the same call takes 118 us
 // without any, 185 with the products alone, 209 with the decoding too: what is left besides the products is the chain from
 // one role to the next, several times per 128 rows, and the softmax's part of it. 128 columns a softmax thread: 280 to 298;
