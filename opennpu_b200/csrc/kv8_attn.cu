@@ -17,8 +17,9 @@
 //    one token over 131001 rows 65.0 -> 49.5 us, 484 warp instructions per 16 rows before.
 //  * weights: w = 2^(x - m) * s_v * c, rounded to fp16 (one part for bf16 outputs: 2^-11 of a weight against the output's
 //    2^-8; two parts, 22 bits, for fp32), times V's codes as fp16, exactly (|c| <= 127): 0x64uu is 1024 + uu. c is a
-//    query's own and puts the largest weight that it has had at 2^6 to 2^10: what it does not see or what weighs nothing does
-//    not count, however large its s_v is. Weights 2^20 below that one (two parts: 2^9) lose bits, 2^-31 of it at most.
+//    query's own: its largest weight so far stands at 2^6 or more, and is brought back to 2^6 before one could pass 2^16. What
+//    it does not see or what weighs nothing does not count, however large its s_v is. Weights 2^20 below the largest (two
+//    parts: 2^9) lose bits, 2^-31 of the largest at most.
 //  * m is a reference within 2^6 (no mask) or e^4 (mask) of the running maximum, raised only when a score
 //    passes it by more: the accumulators are rescaled a few times a sequence, not every step. With a mask
 //    scores stay in natural units, x - m is formed first, so masks of the lowest finite value stay finite.

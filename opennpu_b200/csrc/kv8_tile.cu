@@ -328,13 +328,15 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                     if (__any_sync(0xffffffffu, a != 1.f)) rescale_o(a);
                 }
                 float sh[4];                                     // a group's log2(s_v) - d + kTop
-                bool near = true;                                // and weights that do not underflow in the sum
+                bool alike = true, above = true;                 // and whether 2^sh is a number that loses nothing, and 2^-sh
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     sh[g] = lg[g] - (d == -INFINITY ? 0.f : d) + kTop;
-                    near &= sh[g] > -80.f;
+                    alike &= sh[g] < 100.f;
+                    above &= sh[g] > -80.f;
                 }
-                const bool usual = clear && __all_sync(0xffffffffu, near);
+                const bool usual = clear && __all_sync(0xffffffffu, above);
+                alike = __all_sync(0xffffffffu, alike);
                 // the weights of this half
                 if (live) {
 #pragma unroll
@@ -360,16 +362,27 @@ __global__ void __launch_bounds__(TileSizes<DP, QT>::threads, 1)
                                 }
                                 l = fmaf(s0 + s1, ex2(-sh[2 * ch + g]), l);
                             } else {
-                                const float at = sh[2 * ch + g];
+                                const float at = sh[2 * ch + g], wg = ex2(at);
                                 const int col = r0 + 64 * hf + 32 * ch + 16 * g;
+                                // a row that is not seen weighs nothing, even where its scale is NaN
+                                if (alike) {
 #pragma unroll
-                                for (int k = 0; k < 16; k += 2) {
-                                    const float x0 = score(s[16 * g + k], f, col + k), x1 = score(s[16 * g + k + 1], f, col + k + 1);
-                                    s0 += ex2((x0 - m) * U);
-                                    s1 += ex2((x1 - m) * U);
-                                    // a row that is not seen weighs nothing, even where its scale is NaN
-                                    ph[8 * g + k / 2] = pack_h2(x0 == -INFINITY ? 0.f : ex2(fmaf(x0 - m, U, at)),
-                                                                x1 == -INFINITY ? 0.f : ex2(fmaf(x1 - m, U, at)));
+                                    for (int k = 0; k < 16; k += 2) {
+                                        const float x0 = score(s[16 * g + k], f, col + k), x1 = score(s[16 * g + k + 1], f, col + k + 1);
+                                        const float e0 = ex2((x0 - m) * U), e1 = ex2((x1 - m) * U);
+                                        s0 += e0;
+                                        s1 += e1;
+                                        ph[8 * g + k / 2] = pack_h2(x0 == -INFINITY ? 0.f : e0 * wg, x1 == -INFINITY ? 0.f : e1 * wg);
+                                    }
+                                } else {
+#pragma unroll
+                                    for (int k = 0; k < 16; k += 2) {
+                                        const float x0 = score(s[16 * g + k], f, col + k), x1 = score(s[16 * g + k + 1], f, col + k + 1);
+                                        s0 += ex2((x0 - m) * U);
+                                        s1 += ex2((x1 - m) * U);
+                                        ph[8 * g + k / 2] = pack_h2(x0 == -INFINITY ? 0.f : ex2(fmaf(x0 - m, U, at)),
+                                                                    x1 == -INFINITY ? 0.f : ex2(fmaf(x1 - m, U, at)));
+                                    }
                                 }
                                 l += s0 + s1;
                             }

@@ -123,6 +123,35 @@ def test_scores_and_value_scales_that_grow_in_the_same_tile(D, T):
     assert status() == 0
 
 
+# ---------------------------------------------------------------- many steps of the online softmax
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("B,T,Hq,H,D,S,dtype", [
+    (1, 1, 8, 2, 128, 120000, "bf16"), (1, 1, 8, 2, 128, 120000, "fp32"), (1, 1, 8, 1, 64, 250000, "bf16"),
+    (1, 1, 8, 1, 64, 250000, "fp32"), (1, 1, 8, 2, 256, 70000, "bf16"), (1, 1, 8, 2, 256, 70000, "fp32"),
+    (2, 3, 8, 2, 128, 70000, "bf16"), (2, 3, 8, 2, 128, 70000, "fp32"), (1, 4, 16, 1, 64, 200000, "bf16"),
+    (1, 4, 16, 1, 64, 200000, "fp32"), (1, 20, 8, 1, 256, 40000, "bf16"), (1, 30, 8, 2, 192, 40000, "fp32"),
+    (1, 25, 8, 2, 128, 60000, "bf16"), (1, 25, 8, 2, 80, 60000, "bf16"), (1, 70, 8, 2, 128, 40000, "bf16"),
+    (2, 130, 8, 2, 64, 20000, "bf16"), (2, 90, 16, 8, 128, 16384, "bf16")])
+def test_long_runs(B, T, Hq, H, D, S, dtype, masked):
+    """Scores that rise and fall by some 2^60 along the rows and value scales that double four times over and over: references and
+    factors move in most steps, and each warp and CTA takes several. With masks over a third of the rows and sinks."""
+    block = 16
+    cache = rand_cache(S, B, H, S, D, block)
+    wave = (torch.arange(S, device="cuda") % 3000 - 1500).abs() / 750 - 1
+    cache[0].copy_((cache[0] * 0.3 + 85 * wave[:, None]).round())
+    cache[3][:] *= 50 * sawtooth(cache[3].shape[2], 5, 1, 5)
+    q = (rand_q(T, (B, T, Hq, D), dtype).float().abs() * (128 / D) ** 0.5).to(DT[dtype])
+    mask = sinks = None
+    if masked:
+        g = torch.Generator(device="cuda").manual_seed(T)
+        mask = torch.randn(B, T, S, device="cuda", generator=g)
+        mask.masked_fill_(torch.rand(B, T, S, device="cuda", generator=g) < 0.3, -np.inf)
+        sinks = torch.randn(Hq, device="cuda", generator=g)
+    y = KVCache8.from_tensors(*cache, block).attn(q, i32([S - T] * B), mask=mask, sinks=sinks)
+    check(y, cache, block, some_queries(B, T, Hq), q, [S - T] * B, mask, sinks)
+    assert status() == 0
+
+
 # ---------------------------------------------------------------- value scales far apart
 @pytest.mark.parametrize("T,D", [(20, 128), (20, 64), (60, 128), (60, 64)])
 @pytest.mark.parametrize("tiny", [1e-38, 1e-41, 1e-44])
