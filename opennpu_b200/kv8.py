@@ -28,6 +28,7 @@ class KVCache8:
     Calls run on the current stream (or ``stream``), asynchronously."""
 
     def __init__(self, batch, heads, rows, dim, block=32, device="cuda"):
+        _need(block in (16, 32, 64), "block: 16, 32 or 64")
         nb = -(-rows // block)
         z = dict(device=device)
         self._bind(torch.zeros(batch, heads, rows, dim, dtype=torch.int8, **z),

@@ -65,3 +65,9 @@ def test_a_cache_on_another_device_than_the_current_one_is_refused(monkeypatch):
     k, s = FakeCuda(torch.int8, 2, 4, 100, 64), FakeCuda(torch.float32, 2, 4, 4)
     with pytest.raises(L.OnpuError, match="current device"):
         kv8.KVCache8.from_tensors(k, k, s, s)
+
+
+@pytest.mark.parametrize("block", [0, 8, -32, 48, None])
+def test_a_bad_block_is_refused_before_anything_is_allocated(block):
+    with pytest.raises(L.OnpuError, match="block"):
+        kv8.KVCache8(1, 1, 32, 64, block=block)
