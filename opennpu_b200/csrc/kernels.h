@@ -274,7 +274,7 @@ struct Kv8AttnParams {
     float scale;
     void *ws;                         // kv8_attn_ws_bytes, 16-byte aligned
 };
-int64_t kv8_attn_ws_bytes(int Hq, int Hkv, int D, int T, bool bf16);
+int64_t kv8_attn_ws_bytes(int Hq, int Hkv, int D, int T, bool bf16);     // < 0: a lookup on the device failed
 cudaError_t kv8_attn_launch(const Kv8AttnParams &p, bool bf16, cudaStream_t stream);
 // its kernel for many bf16 queries a kv head, D <= 128 (kv8_tile.cu): query tile, rows of a unit and CTAs of its list
 int kv8_tile_queries(int64_t queries);
